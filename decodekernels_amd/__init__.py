@@ -9,7 +9,9 @@ Same public API as DecodeKernels' ``decode_kernels`` package
 ``reshape_and_cache`` add the two steps around attention that the reference
 leaves to vLLM (vLLM's signatures); ``rotary_embedding_and_cache`` runs both
 in one launch. ``gemm_add_rms_norm`` and ``gemm_rotary_embedding_and_cache``
-fuse a decode GEMM with the op that consumes its output.
+fuse a decode GEMM with the op that consumes its output. ``build_slot_mapping``,
+``qk_norm_rotary_embedding(_and_cache)`` and ``paged_attention_varlen`` run the
+attention step of a batch whose sequences bring any number of new tokens.
 """
 
 from .ops import (
@@ -18,6 +20,7 @@ from .ops import (
     SUPPORTED_FP8_HEAD_DIMS,
     SUPPORTED_HEAD_DIMS,
     alloc_workspace,
+    build_slot_mapping,
     fused_add_rms_norm,
     gemm,
     gemm_add_rms_norm,
@@ -25,6 +28,9 @@ from .ops import (
     is_available,
     num_partitions,
     paged_attention_decode,
+    paged_attention_varlen,
+    qk_norm_rotary_embedding,
+    qk_norm_rotary_embedding_and_cache,
     reshape_and_cache,
     rms_norm,
     rotary_embedding,
@@ -38,6 +44,7 @@ __all__ = [
     "SUPPORTED_FP8_HEAD_DIMS",
     "SUPPORTED_HEAD_DIMS",
     "alloc_workspace",
+    "build_slot_mapping",
     "fused_add_rms_norm",
     "gemm",
     "gemm_add_rms_norm",
@@ -45,6 +52,9 @@ __all__ = [
     "is_available",
     "num_partitions",
     "paged_attention_decode",
+    "paged_attention_varlen",
+    "qk_norm_rotary_embedding",
+    "qk_norm_rotary_embedding_and_cache",
     "reshape_and_cache",
     "rms_norm",
     "rotary_embedding",

@@ -109,6 +109,79 @@ class CacheWriteParams(ctypes.Structure):
     ]
 
 
+class SlotMappingParams(ctypes.Structure):
+    """Mirror of ``dk_slot_mapping_params``."""
+
+    _fields_ = [
+        ("query_start_loc", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("free_blocks", ctypes.c_void_p),
+        ("positions", ctypes.c_void_p),
+        ("slot_mapping", ctypes.c_void_p),
+        ("num_new_blocks", ctypes.c_void_p),
+        ("bt_stride", ctypes.c_int64),
+        ("num_seqs", ctypes.c_int32),
+        ("num_tokens", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("num_free_blocks", ctypes.c_int32),
+    ]
+
+
+class QkNormParams(ctypes.Structure):
+    """Mirror of ``dk_qk_norm_params``."""
+
+    _fields_ = [
+        ("q_weight", ctypes.c_void_p),
+        ("k_weight", ctypes.c_void_p),
+        ("query_out", ctypes.c_void_p),
+        ("key_out", ctypes.c_void_p),
+        ("qo_stride_token", ctypes.c_int64),
+        ("qo_stride_head", ctypes.c_int64),
+        ("ko_stride_token", ctypes.c_int64),
+        ("ko_stride_head", ctypes.c_int64),
+        ("eps", ctypes.c_float),
+    ]
+
+
+class VarlenAttnParams(ctypes.Structure):
+    """Mirror of ``dk_varlen_attn_params``."""
+
+    _fields_ = [
+        ("out", ctypes.c_void_p),
+        ("q", ctypes.c_void_p),
+        ("k_cache", ctypes.c_void_p),
+        ("v_cache", ctypes.c_void_p),
+        ("block_tables", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("query_start_loc", ctypes.c_void_p),
+        ("prefix_lens", ctypes.c_void_p),
+        ("alibi_slopes", ctypes.c_void_p),
+        ("q_stride_token", ctypes.c_int64),
+        ("q_stride_head", ctypes.c_int64),
+        ("out_stride_token", ctypes.c_int64),
+        ("out_stride_head", ctypes.c_int64),
+        ("k_stride_block", ctypes.c_int64),
+        ("k_stride_token", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v_stride_block", ctypes.c_int64),
+        ("v_stride_token", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("bt_stride", ctypes.c_int64),
+        ("num_tokens", ctypes.c_int32),
+        ("num_seqs", ctypes.c_int32),
+        ("num_q_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("max_blocks", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("softcap", ctypes.c_float),
+    ]
+
+
 _LIB: ctypes.CDLL | None = None
 
 _SIGNATURES = {
@@ -194,6 +267,34 @@ _SIGNATURES = {
         [ctypes.c_int] + [ctypes.c_void_p] * 4 + [ctypes.c_int] * 6
         + [ctypes.POINTER(RotaryParams), ctypes.POINTER(CacheWriteParams), ctypes.c_float, ctypes.c_float,
            ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "dk_build_slot_mapping": (ctypes.c_int, [ctypes.POINTER(SlotMappingParams), ctypes.c_void_p]),
+    "dk_qk_norm_rotary_embedding": (
+        ctypes.c_int,
+        [ctypes.POINTER(RotaryParams), ctypes.POINTER(QkNormParams), ctypes.c_int, ctypes.c_void_p],
+    ),
+    "dk_qk_norm_rotary_embedding_and_cache": (
+        ctypes.c_int,
+        [ctypes.POINTER(RotaryParams), ctypes.POINTER(QkNormParams), ctypes.POINTER(CacheWriteParams), ctypes.c_int]
+        + [ctypes.c_void_p],
+    ),
+    "dk_qk_norm_rotary_embedding_and_cache_fp8": (
+        ctypes.c_int,
+        [ctypes.POINTER(RotaryParams), ctypes.POINTER(QkNormParams), ctypes.POINTER(CacheWriteParams), ctypes.c_int]
+        + [ctypes.c_float, ctypes.c_float, ctypes.c_void_p],
+    ),
+    "dk_paged_attention_varlen_workspace_bytes": (
+        ctypes.c_int64,
+        [ctypes.POINTER(VarlenAttnParams), ctypes.c_int, ctypes.c_int, ctypes.c_int],
+    ),
+    "dk_paged_attention_varlen": (
+        ctypes.c_int,
+        [ctypes.POINTER(VarlenAttnParams)] + [ctypes.c_int] * 4 + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
+    ),
+    "dk_paged_attention_varlen_fp8": (
+        ctypes.c_int,
+        [ctypes.POINTER(VarlenAttnParams)] + [ctypes.c_int] * 4 + [ctypes.c_float, ctypes.c_float]
+        + [ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p],
     ),
     "dk_last_error": (ctypes.c_char_p, []),
     "dk_error_string": (ctypes.c_char_p, [ctypes.c_int]),
@@ -325,4 +426,63 @@ def cache_write_params(key, value, key_cache, value_cache, slot_mapping) -> Cach
     p.vc_stride_block, p.vc_stride_token, p.vc_stride_head = value_cache.stride()[:3]
     p.num_tokens = slot_mapping.numel()
     p.num_blocks, p.block_size, p.num_kv_heads, p.head_size = key_cache.shape
+    return p
+
+
+def qk_norm_params(q_weight, k_weight, eps, head_size, query_out, key_out=None) -> QkNormParams:
+    """Fills ``dk_qk_norm_params`` from tensors; ``query_out`` / ``key_out`` are
+    [tokens, heads * head_size] or [tokens, heads, head_size]."""
+    p = QkNormParams()
+    p.q_weight, p.k_weight = q_weight.data_ptr(), k_weight.data_ptr()
+    p.query_out = query_out.data_ptr()
+    p.qo_stride_token, p.qo_stride_head = _token_head_strides(query_out, head_size)
+    if key_out is not None:
+        p.key_out = key_out.data_ptr()
+        p.ko_stride_token, p.ko_stride_head = _token_head_strides(key_out, head_size)
+    p.eps = eps
+    return p
+
+
+def slot_mapping_params(
+    query_start_loc, seq_lens, block_tables, block_size, positions, slot_mapping, free_blocks=None, num_new_blocks=None
+) -> SlotMappingParams:
+    """Fills ``dk_slot_mapping_params`` from tensors."""
+    p = SlotMappingParams()
+    p.query_start_loc, p.seq_lens = query_start_loc.data_ptr(), seq_lens.data_ptr()
+    p.block_tables = block_tables.data_ptr()
+    p.positions, p.slot_mapping = positions.data_ptr(), slot_mapping.data_ptr()
+    if free_blocks is not None:
+        p.free_blocks, p.num_free_blocks = free_blocks.data_ptr(), free_blocks.numel()
+    if num_new_blocks is not None:
+        p.num_new_blocks = num_new_blocks.data_ptr()
+    p.bt_stride = block_tables.stride(0)
+    p.num_seqs, p.num_tokens = query_start_loc.numel() - 1, positions.numel()
+    p.block_size, p.max_blocks = block_size, block_tables.shape[1]
+    return p
+
+
+def varlen_attn_params(
+    out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, scale, window=0, softcap=0.0, alibi_slopes=None,
+    prefix_lens=None
+) -> VarlenAttnParams:
+    """Fills ``dk_varlen_attn_params`` from tensors (strides in elements)."""
+    p = VarlenAttnParams()
+    p.out, p.q = out.data_ptr(), q.data_ptr()
+    p.k_cache, p.v_cache = k_cache.data_ptr(), v_cache.data_ptr()
+    p.block_tables, p.seq_lens = block_tables.data_ptr(), seq_lens.data_ptr()
+    p.query_start_loc = query_start_loc.data_ptr()
+    if prefix_lens is not None:
+        p.prefix_lens = prefix_lens.data_ptr()
+    if alibi_slopes is not None:
+        p.alibi_slopes = alibi_slopes.data_ptr()
+    p.q_stride_token, p.q_stride_head = q.stride(0), q.stride(1)
+    p.out_stride_token, p.out_stride_head = out.stride(0), out.stride(1)
+    p.k_stride_block, p.k_stride_token, p.k_stride_head = k_cache.stride()[:3]
+    p.v_stride_block, p.v_stride_token, p.v_stride_head = v_cache.stride()[:3]
+    p.bt_stride = block_tables.stride(0)
+    p.num_tokens, p.num_q_heads, _ = q.shape
+    p.num_seqs = query_start_loc.numel() - 1
+    p.num_blocks, p.block_size, p.num_kv_heads, _ = k_cache.shape
+    p.max_blocks = block_tables.shape[1]
+    p.window, p.scale, p.softcap = window, scale, softcap
     return p

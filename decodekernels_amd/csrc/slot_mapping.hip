@@ -1,0 +1,189 @@
+// Positions, cache slots and new cache blocks of the tokens of a ragged batch,
+// from the request lengths alone (gfx950): the step before the cache write of
+// a serving engine, kept on the GPU so that no length has to reach the host.
+//
+// Sequence s brings n_s = start[s + 1] - start[s] tokens, which end a sequence
+// of len_s; c_s = len_s - n_s tokens are in the cache already. With cache
+// blocks of b tokens it holds ceil(c_s / b) blocks and needs ceil(len_s / b);
+// the blocks in between are taken from the free list in the order of the
+// sequences:
+//   first_s = sum over i < s of (ceil(len_i / b) - ceil(c_i / b)),
+//   token t of s: position c_s + t - start[s], block position / b of s, which is
+//   block_tables[s][.] or, past the blocks held, free_blocks[first_s + . - held].
+//
+// The work is 16 bytes written per token after two dependent reads, so the
+// call costs a launch and two round trips. Every workgroup takes its own
+// tokens and redoes the prefix sum over the sequences (8 bytes each, from L2)
+// rather than wait for another launch. The token that begins a new block
+// enters it into the table, so no pass over the tables is needed.
+#include "../../include/decodekernels_amd.h"
+#include "dk_device.h"
+#include "dk_host.h"
+
+namespace dk {
+namespace slots {
+
+constexpr int kThreads = 256;
+constexpr int kSeqsPerThread = 4;
+constexpr int kChunk = kThreads * kSeqsPerThread;  // sequences whose prefix sum is in LDS at once
+
+struct KParams {
+  const int32_t* starts;
+  const int32_t* lens;
+  int32_t* tables;
+  const int32_t* free_blocks;
+  int64_t* positions;
+  int64_t* slots;
+  int32_t* num_new;
+  int64_t bt_stride;
+  int num_seqs, num_tokens, block_size, max_blocks, num_free;
+};
+
+__global__ __launch_bounds__(kThreads) void slot_mapping_kernel(const KParams p) {
+  __shared__ int start[kChunk + 1];
+  __shared__ int len[kChunk];
+  __shared__ int first[kChunk];  // free blocks taken before each sequence
+  __shared__ int wave_total[kThreads / kWave];
+  const int tid = threadIdx.x;
+  const int lane = tid % kWave;
+  const int wave = tid / kWave;
+  const int b = p.block_size;
+  const int t = static_cast<int>(blockIdx.x) * kThreads + tid;
+  const int t_first = static_cast<int>(blockIdx.x) * kThreads;
+  const int t_last = min(t_first + kThreads, p.num_tokens) - 1;
+  const bool totals = blockIdx.x == 0 && p.num_new != nullptr;  // this workgroup walks all sequences
+  // Rows that no sequence owns keep -1: no token, for the steps that follow.
+  int64_t position = -1, slot = -1;
+  int base = 0;  // free blocks taken before this chunk
+  for (int s0 = 0; s0 < p.num_seqs; s0 += kChunk) {
+    const int count = min(kChunk, p.num_seqs - s0);
+    int taken[kSeqsPerThread];
+    int sum = 0;
+    int st[kSeqsPerThread + 1], ln[kSeqsPerThread];
+#pragma unroll
+    for (int i = 0; i <= kSeqsPerThread; ++i) st[i] = p.starts[min(s0 + tid * kSeqsPerThread + i, p.num_seqs)];
+#pragma unroll
+    for (int i = 0; i < kSeqsPerThread; ++i) ln[i] = p.lens[min(s0 + tid * kSeqsPerThread + i, p.num_seqs - 1)];
+#pragma unroll
+    for (int i = 0; i < kSeqsPerThread; ++i) {
+      const int s = tid * kSeqsPerThread + i;
+      const int n = min(max(st[i + 1] - st[i], 0), p.num_tokens);
+      const int cached = max(ln[i] - n, 0);
+      const int held = cached / b + (cached % b != 0);
+      const int need = ln[i] > 0 ? ln[i] / b + (ln[i] % b != 0) : 0;
+      taken[i] = s < count && n > 0 ? max(need - held, 0) : 0;
+      sum += taken[i];
+    }
+    int scan = sum;  // inclusive over the wave's lanes
+#pragma unroll
+    for (int off = 1; off < kWave; off <<= 1) {
+      const int v = __shfl_up(scan, off, kWave);
+      if (lane >= off) scan += v;
+    }
+    __syncthreads();  // the previous chunk has been read
+    if (lane == kWave - 1) wave_total[wave] = scan;
+#pragma unroll
+    for (int i = 0; i < kSeqsPerThread; ++i) {
+      const int s = tid * kSeqsPerThread + i;
+      if (s < count) {
+        start[s] = st[i];
+        len[s] = ln[i];
+        if (s == count - 1) start[count] = st[i + 1];
+      }
+    }
+    __syncthreads();
+    int before = base + scan - sum;
+    int total = 0;
+    for (int w = 0; w < kThreads / kWave; ++w) {
+      if (w < wave) before += wave_total[w];
+      total += wave_total[w];
+    }
+#pragma unroll
+    for (int i = 0; i < kSeqsPerThread; ++i) {
+      const int s = tid * kSeqsPerThread + i;
+      if (s < count) first[s] = before;
+      before += taken[i];
+    }
+    base += total;
+    __syncthreads();
+    if (t < p.num_tokens && t >= start[0] && t < start[count]) {
+      int lo = 0, hi = count;  // the last sequence that starts at or before t
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (start[mid] <= t) lo = mid;
+        else hi = mid;
+      }
+      const int n = min(max(start[lo + 1] - start[lo], 0), p.num_tokens);
+      const int cached = len[lo] - n;
+      const int pos = cached + t - start[lo];
+      if (pos >= 0) {  // a length below its new tokens leaves the first ones without a place
+        position = pos;
+        const int held = max(cached, 0) / b + (max(cached, 0) % b != 0);
+        const int blk = pos / b;
+        int page = -1;
+        int32_t* entry = p.tables + (s0 + lo) * p.bt_stride + blk;
+        if (blk < p.max_blocks) {
+          if (blk < held || p.free_blocks == nullptr) {
+            page = *entry;
+          } else {
+            const int64_t at = static_cast<int64_t>(first[lo]) + blk - held;
+            if (at < p.num_free) {
+              page = p.free_blocks[at];
+              if (pos - blk * b == 0) *entry = page;
+            }
+          }
+        }
+        if (page >= 0) slot = static_cast<int64_t>(page) * b + (pos - blk * b);
+      }
+    }
+    if (!totals && t_last < start[count]) break;  // the same for the whole workgroup
+  }
+  if (t < p.num_tokens) {
+    p.positions[t] = position;
+    p.slots[t] = slot;
+  }
+  if (totals && tid == 0) *p.num_new = base;
+}
+
+}  // namespace slots
+}  // namespace dk
+
+extern "C" int dk_build_slot_mapping(const dk_slot_mapping_params* a, void* stream) {
+  using namespace dk;
+  clear_error();
+  const char* op = "build_slot_mapping";
+  if (a == nullptr) return fail("%s: params must not be NULL", op);
+  if (a->num_seqs < 0 || a->num_tokens < 0 || a->max_blocks < 0 || a->num_free_blocks < 0)
+    return fail("%s: sizes must be non-negative", op);
+  if (a->block_size <= 0) return fail("%s: block_size must be positive", op);
+  if (a->num_seqs > (1 << 30) || a->num_tokens > (1 << 30)) return fail("%s: too many sequences or tokens", op);
+  if (a->num_tokens == 0 && a->num_new_blocks == nullptr) return hipSuccess;
+  if (a->num_seqs > 0 && (a->query_start_loc == nullptr || a->seq_lens == nullptr))
+    return fail("%s: query_start_loc and seq_lens must not be NULL", op);
+  if (a->num_seqs > 0 && a->max_blocks > 0 && a->block_tables == nullptr)
+    return fail("%s: block_tables must not be NULL", op);
+  if (a->num_tokens > 0 && (a->positions == nullptr || a->slot_mapping == nullptr))
+    return fail("%s: positions and slot_mapping must not be NULL", op);
+  if (a->num_seqs > 1 && a->bt_stride < a->max_blocks)
+    return fail("%s: block-table rows of %d entries overlap (row stride %lld)", op, static_cast<int>(a->max_blocks),
+                static_cast<long long>(a->bt_stride));
+  if (a->free_blocks == nullptr && a->num_free_blocks > 0) return fail("%s: free_blocks must not be NULL", op);
+  slots::KParams kp{};
+  kp.starts = a->query_start_loc;
+  kp.lens = a->seq_lens;
+  kp.tables = a->block_tables;
+  kp.free_blocks = a->free_blocks;
+  kp.positions = a->positions;
+  kp.slots = a->slot_mapping;
+  kp.num_new = a->num_new_blocks;
+  kp.bt_stride = a->bt_stride;
+  kp.num_seqs = a->num_seqs;
+  kp.num_tokens = a->num_tokens;
+  kp.block_size = a->block_size;
+  kp.max_blocks = a->max_blocks;
+  kp.num_free = a->num_free_blocks;
+  const int64_t groups = ceil_div64(a->num_tokens, slots::kThreads);
+  const dim3 grid(static_cast<unsigned>(groups > 0 ? groups : 1)), block(slots::kThreads);
+  hipLaunchKernelGGL(slots::slot_mapping_kernel, grid, block, 0, static_cast<hipStream_t>(stream), kp);
+  return static_cast<int>(hipGetLastError());
+}

@@ -582,6 +582,305 @@ void gemm_tn_rotary_embedding_and_cache_fp8(at::Tensor& qkv, const at::Tensor& a
 }
 
 // ---------------------------------------------------------------------------
+// The attention step of a ragged batch (sequences that bring any number of new
+// tokens): slot maps, head norms with rotation and cache write, attention. No
+// counterparts in the reference.
+// ---------------------------------------------------------------------------
+namespace {
+
+void check_int32(const at::Tensor& t, int64_t at_least, const at::Tensor& like, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 1 && t.is_contiguous(), what,
+              " must be a contiguous 1-D int32 tensor");
+  TORCH_CHECK(t.size(0) >= at_least, what, " must have at least ", at_least, " entries, got ", t.size(0));
+  TORCH_CHECK(t.device() == like.device(), what, ": tensors must be on the same device");
+}
+
+// Rows of a block table that the sequences use.
+void check_block_tables(const at::Tensor& t, int64_t num_seqs, const at::Tensor& like, const char* op) {
+  TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 2 && (t.stride(1) == 1 || t.size(1) <= 1),
+              op, ": block_tables must be a 2-D int32 tensor with a contiguous last dimension");
+  TORCH_CHECK(t.size(0) >= num_seqs, op, ": block_tables must have at least ", num_seqs, " rows");
+  TORCH_CHECK(t.size(1) < (int64_t{1} << 31), op, ": sizes must fit in 32 bits");
+  TORCH_CHECK(t.device() == like.device(), op, ": tensors must be on the same device");
+}
+
+int64_t num_seqs_of(const at::Tensor& query_start_loc, const char* op) {
+  TORCH_CHECK(query_start_loc.is_cuda(), op, ": query_start_loc must be on CUDA");
+  TORCH_CHECK(query_start_loc.scalar_type() == at::kInt && query_start_loc.dim() == 1 && query_start_loc.is_contiguous() &&
+                  query_start_loc.size(0) >= 1,
+              op, ": query_start_loc must be a contiguous 1-D int32 tensor of num_seqs + 1 entries");
+  TORCH_CHECK(query_start_loc.size(0) <= (int64_t{1} << 30), op, ": sizes must fit in 32 bits");
+  return query_start_loc.size(0) - 1;
+}
+
+}  // namespace
+
+void build_slot_mapping(const at::Tensor& query_start_loc, const at::Tensor& seq_lens, at::Tensor& block_tables,
+                        int64_t block_size, const std::optional<at::Tensor>& free_blocks, at::Tensor& positions,
+                        at::Tensor& slot_mapping, const std::optional<at::Tensor>& num_new_blocks) {
+  const char* op = "build_slot_mapping";
+  const int64_t S = num_seqs_of(query_start_loc, op);
+  check_int32(seq_lens, S, query_start_loc, "build_slot_mapping(seq_lens)");
+  check_block_tables(block_tables, S, query_start_loc, op);
+  TORCH_CHECK(block_size > 0 && block_size < (int64_t{1} << 31), op, ": block_size must be positive");
+  for (const at::Tensor* t : {&positions, &slot_mapping}) {
+    TORCH_CHECK(t->scalar_type() == at::ScalarType::Long && t->dim() == 1 && t->is_contiguous() &&
+                    t->device() == query_start_loc.device(),
+                op, ": positions and slot_mapping must be contiguous 1-D int64 tensors on query_start_loc's device");
+  }
+  TORCH_CHECK(positions.size(0) == slot_mapping.size(0), op, ": positions and slot_mapping must have the same size");
+  TORCH_CHECK(positions.size(0) <= (int64_t{1} << 30), op, ": sizes must fit in 32 bits");
+  dk_slot_mapping_params p{};
+  if (free_blocks.has_value()) {
+    check_int32(*free_blocks, 0, query_start_loc, "build_slot_mapping(free_blocks)");
+    TORCH_CHECK(free_blocks->size(0) < (int64_t{1} << 31), op, ": sizes must fit in 32 bits");
+    p.num_free_blocks = static_cast<int32_t>(free_blocks->size(0));
+    // An empty list is a list all the same, not the absence of one.
+    p.free_blocks = p.num_free_blocks > 0 ? free_blocks->data_ptr<int32_t>() : query_start_loc.data_ptr<int32_t>();
+  }
+  if (num_new_blocks.has_value()) {
+    check_int32(*num_new_blocks, 1, query_start_loc, "build_slot_mapping(num_new_blocks)");
+    p.num_new_blocks = num_new_blocks->data_ptr<int32_t>();
+  }
+  p.query_start_loc = query_start_loc.data_ptr<int32_t>();
+  p.seq_lens = seq_lens.data_ptr<int32_t>();
+  p.block_tables = block_tables.data_ptr<int32_t>();
+  p.positions = positions.data_ptr<int64_t>();
+  p.slot_mapping = slot_mapping.data_ptr<int64_t>();
+  p.bt_stride = block_tables.stride(0);
+  p.num_seqs = static_cast<int32_t>(S);
+  p.num_tokens = static_cast<int32_t>(positions.size(0));
+  p.block_size = static_cast<int32_t>(block_size);
+  p.max_blocks = static_cast<int32_t>(block_tables.size(1));
+  const DeviceGuard guard(query_start_loc.device());
+  check_status(dk_build_slot_mapping(&p, stream_of(query_start_loc)), op);
+}
+
+namespace {
+
+// Checked dk_qk_norm_params; the inputs were checked by rotary_params.
+dk_qk_norm_params qk_norm_params(const at::Tensor& query, const at::Tensor& key, const at::Tensor& q_weight,
+                                 const at::Tensor& k_weight, double eps, int64_t head_size, at::Tensor& query_out,
+                                 at::Tensor* key_out, const char* op) {
+  for (const at::Tensor* w : {&q_weight, &k_weight}) {
+    check_same(query, *w, "query/weight");
+    TORCH_CHECK(w->dim() == 1 && w->size(0) == head_size && w->is_contiguous(), op,
+                ": q_weight and k_weight must be [head_size]");
+  }
+  dk_qk_norm_params n{};
+  n.q_weight = q_weight.data_ptr();
+  n.k_weight = k_weight.data_ptr();
+  check_same(query, query_out, "query/query_out");
+  TORCH_CHECK(query_out.size(0) == query.size(0), op, ": query_out must have one row per position");
+  std::tie(n.qo_stride_token, n.qo_stride_head) = token_head_strides(query_out, head_size, "qk_norm(query_out)");
+  TORCH_CHECK(heads_of(query_out, head_size) == heads_of(query, head_size), op, ": query_out must have query's heads");
+  n.query_out = query_out.data_ptr();
+  if (key_out != nullptr) {
+    check_same(key, *key_out, "key/key_out");
+    TORCH_CHECK(key_out->size(0) == key.size(0), op, ": key_out must have one row per position");
+    std::tie(n.ko_stride_token, n.ko_stride_head) = token_head_strides(*key_out, head_size, "qk_norm(key_out)");
+    TORCH_CHECK(heads_of(*key_out, head_size) == heads_of(key, head_size), op, ": key_out must have key's heads");
+    n.key_out = key_out->data_ptr();
+  }
+  n.eps = static_cast<float>(eps);
+  return n;
+}
+
+// rotary_params writes through its tensors in place; these ops only read them.
+dk_rotary_params qk_inputs(const at::Tensor& positions, const at::Tensor& query, const at::Tensor& key,
+                           int64_t head_size, const at::Tensor& cos_sin_cache, bool is_neox, int& dt) {
+  TORCH_CHECK(query.dim() >= 2 && key.dim() >= 2,
+              "qk_norm: expected [tokens, heads * head_size] or [tokens, heads, head_size]");
+  TORCH_CHECK(head_size > 0 && head_size < (int64_t{1} << 31), "qk_norm: head_size must be positive");
+  TORCH_CHECK(query.size(0) < (int64_t{1} << 31) && cos_sin_cache.numel() > 0 &&
+                  cos_sin_cache.size(0) < (int64_t{1} << 31),
+              "qk_norm: sizes must fit in 32 bits and the table must not be empty");
+  at::Tensor q = query;
+  return rotary_params(positions, q, key, head_size, cos_sin_cache, is_neox, dt);
+}
+
+void qk_norm_and_cache(const at::Tensor& positions, const at::Tensor& query, const at::Tensor& key,
+                       const at::Tensor& value, const at::Tensor& q_weight, const at::Tensor& k_weight, double eps,
+                       int64_t head_size, const at::Tensor& cos_sin_cache, bool is_neox, at::Tensor& key_cache,
+                       at::Tensor& value_cache, const at::Tensor& slot_mapping, at::Tensor& query_out, bool fp8,
+                       double k_scale, double v_scale, const char* op) {
+  int dt = 0, dt2 = 0;
+  const dk_rotary_params r = qk_inputs(positions, query, key, head_size, cos_sin_cache, is_neox, dt);
+  TORCH_CHECK(value.dim() >= 2 && key_cache.dim() == 4 && key_cache.size(3) == head_size, op,
+              ": cache head_size must equal head_size");
+  const dk_cache_write_params c = cache_params(key, value, key_cache, value_cache, slot_mapping, dt2, fp8);
+  const dk_qk_norm_params n =
+      qk_norm_params(query, key, q_weight, k_weight, eps, head_size, query_out, nullptr, op);
+  const DeviceGuard guard(query.device());
+  if (fp8) {
+    check_status(dk_qk_norm_rotary_embedding_and_cache_fp8(&r, &n, &c, dt, static_cast<float>(k_scale),
+                                                           static_cast<float>(v_scale), stream_of(query)),
+                 op);
+  } else {
+    check_status(dk_qk_norm_rotary_embedding_and_cache(&r, &n, &c, dt, stream_of(query)), op);
+  }
+}
+
+}  // namespace
+
+void qk_norm_rotary_embedding(const at::Tensor& positions, const at::Tensor& query, const at::Tensor& key,
+                              const at::Tensor& q_weight, const at::Tensor& k_weight, double eps, int64_t head_size,
+                              const at::Tensor& cos_sin_cache, bool is_neox, at::Tensor& query_out,
+                              at::Tensor& key_out) {
+  const char* op = "qk_norm_rotary_embedding";
+  int dt = 0;
+  const dk_rotary_params r = qk_inputs(positions, query, key, head_size, cos_sin_cache, is_neox, dt);
+  const dk_qk_norm_params n =
+      qk_norm_params(query, key, q_weight, k_weight, eps, head_size, query_out, &key_out, op);
+  const DeviceGuard guard(query.device());
+  check_status(dk_qk_norm_rotary_embedding(&r, &n, dt, stream_of(query)), op);
+}
+
+void qk_norm_rotary_embedding_and_cache(const at::Tensor& positions, const at::Tensor& query, const at::Tensor& key,
+                                        const at::Tensor& value, const at::Tensor& q_weight,
+                                        const at::Tensor& k_weight, double eps, int64_t head_size,
+                                        const at::Tensor& cos_sin_cache, bool is_neox, at::Tensor& key_cache,
+                                        at::Tensor& value_cache, const at::Tensor& slot_mapping,
+                                        at::Tensor& query_out) {
+  qk_norm_and_cache(positions, query, key, value, q_weight, k_weight, eps, head_size, cos_sin_cache, is_neox,
+                    key_cache, value_cache, slot_mapping, query_out, false, 1.0, 1.0,
+                    "qk_norm_rotary_embedding_and_cache");
+}
+
+void qk_norm_rotary_embedding_and_cache_fp8(const at::Tensor& positions, const at::Tensor& query,
+                                            const at::Tensor& key, const at::Tensor& value, const at::Tensor& q_weight,
+                                            const at::Tensor& k_weight, double eps, int64_t head_size,
+                                            const at::Tensor& cos_sin_cache, bool is_neox, at::Tensor& key_cache,
+                                            at::Tensor& value_cache, const at::Tensor& slot_mapping,
+                                            at::Tensor& query_out, double k_scale, double v_scale) {
+  qk_norm_and_cache(positions, query, key, value, q_weight, k_weight, eps, head_size, cos_sin_cache, is_neox,
+                    key_cache, value_cache, slot_mapping, query_out, true, k_scale, v_scale,
+                    "qk_norm_rotary_embedding_and_cache_fp8");
+}
+
+namespace {
+
+void varlen_impl(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                 const at::Tensor& block_tables, const at::Tensor& seq_lens, const at::Tensor& query_start_loc,
+                 double scale, int64_t max_query_len, int64_t max_seq_len, int64_t window, double softcap,
+                 const std::optional<at::Tensor>& alibi_slopes, const std::optional<at::Tensor>& prefix_lens, bool fp8,
+                 double k_scale, double v_scale, const char* op) {
+  constexpr int64_t kMost = int64_t{1} << 31;
+  TORCH_CHECK(q.is_cuda(), op, ": q must be a CUDA tensor");
+  TORCH_CHECK(q.dim() == 3 && out.dim() == 3, op, ": q and out must be [num_tokens, num_q_heads, head_dim]");
+  TORCH_CHECK(k_cache.dim() == 4 && v_cache.dim() == 4, op,
+              ": k_cache and v_cache must be [num_blocks, block_size, num_kv_heads, head_dim]");
+  check_same(q, out, "q/out");
+  TORCH_CHECK(out.sizes() == q.sizes(), op, ": out must have the same shape as q");
+  if (fp8) {
+    TORCH_CHECK(k_cache.scalar_type() == at::ScalarType::Float8_e4m3fn &&
+                    v_cache.scalar_type() == at::ScalarType::Float8_e4m3fn,
+                op, ": k_cache and v_cache must be float8_e4m3fn");
+    TORCH_CHECK(k_cache.device() == q.device() && v_cache.device() == q.device(), op,
+                ": tensors must be on the same device");
+  } else {
+    check_same(q, k_cache, "q/k_cache");
+    check_same(q, v_cache, "q/v_cache");
+  }
+  TORCH_CHECK(k_cache.sizes() == v_cache.sizes(), op, ": k_cache and v_cache shapes differ");
+  TORCH_CHECK(k_cache.size(3) == q.size(2), op, ": cache head_dim does not match q");
+  TORCH_CHECK(q.stride(2) == 1 && out.stride(2) == 1 && k_cache.stride(3) == 1 && v_cache.stride(3) == 1, op,
+              ": head_dim must be the contiguous (innermost) dimension");
+  const int64_t S = num_seqs_of(query_start_loc, op);
+  TORCH_CHECK(query_start_loc.device() == q.device(), op, ": tensors must be on the same device");
+  check_int32(seq_lens, S, q, "paged_attention_varlen(seq_lens)");
+  check_block_tables(block_tables, S, q, op);
+  TORCH_CHECK(q.size(0) < kMost && q.size(1) < kMost && k_cache.size(0) < kMost && k_cache.size(1) < kMost &&
+                  k_cache.size(2) < kMost && q.size(2) < kMost,
+              op, ": sizes must fit in 32 bits");
+  TORCH_CHECK(max_query_len >= 0 && max_seq_len >= 0 && max_query_len < kMost && max_seq_len < kMost, op,
+              ": max_query_len and max_seq_len must be non-negative and fit in 32 bits");
+  TORCH_CHECK(window >= 0, op, ": window must be non-negative (0: none)");
+  dk_varlen_attn_params p{};
+  if (alibi_slopes.has_value()) {
+    TORCH_CHECK(alibi_slopes->scalar_type() == at::kFloat && alibi_slopes->dim() == 1 &&
+                    alibi_slopes->size(0) == q.size(1) && alibi_slopes->is_contiguous() &&
+                    alibi_slopes->device() == q.device(),
+                op, ": alibi_slopes must be a contiguous float32 tensor [num_q_heads] on q's device");
+    p.alibi_slopes = alibi_slopes->data_ptr<float>();
+  }
+  if (prefix_lens.has_value()) {
+    check_int32(*prefix_lens, S, q, "paged_attention_varlen(prefix_lens)");
+    p.prefix_lens = prefix_lens->data_ptr<int32_t>();
+  }
+  const int dt = dtype_code(q.scalar_type(), op);
+  p.out = out.data_ptr();
+  p.q = q.data_ptr();
+  p.k_cache = k_cache.data_ptr();
+  p.v_cache = v_cache.data_ptr();
+  p.block_tables = block_tables.data_ptr<int32_t>();
+  p.seq_lens = seq_lens.data_ptr<int32_t>();
+  p.query_start_loc = query_start_loc.data_ptr<int32_t>();
+  p.q_stride_token = q.stride(0);
+  p.q_stride_head = q.stride(1);
+  p.out_stride_token = out.stride(0);
+  p.out_stride_head = out.stride(1);
+  p.k_stride_block = k_cache.stride(0);
+  p.k_stride_token = k_cache.stride(1);
+  p.k_stride_head = k_cache.stride(2);
+  p.v_stride_block = v_cache.stride(0);
+  p.v_stride_token = v_cache.stride(1);
+  p.v_stride_head = v_cache.stride(2);
+  p.bt_stride = block_tables.stride(0);
+  p.num_tokens = static_cast<int32_t>(q.size(0));
+  p.num_seqs = static_cast<int32_t>(S);
+  p.num_q_heads = static_cast<int32_t>(q.size(1));
+  p.num_kv_heads = static_cast<int32_t>(k_cache.size(2));
+  p.block_size = static_cast<int32_t>(k_cache.size(1));
+  p.num_blocks = static_cast<int32_t>(k_cache.size(0));
+  p.max_blocks = static_cast<int32_t>(block_tables.size(1));
+  p.window = static_cast<int32_t>(std::min<int64_t>(window, kMost - 1));
+  p.scale = static_cast<float>(scale);
+  p.softcap = static_cast<float>(softcap);
+  const DeviceGuard guard(q.device());
+  // The partial results of split keys, from the caching allocator as gemm_tn's.
+  const int64_t ws_bytes = dk_paged_attention_varlen_workspace_bytes(&p, static_cast<int>(q.size(2)),
+                                                                     static_cast<int>(max_query_len),
+                                                                     static_cast<int>(max_seq_len));
+  at::Tensor ws;
+  if (ws_bytes > 0) ws = at::empty({ws_bytes / 4}, q.options().dtype(at::kFloat));
+  void* ws_ptr = ws_bytes > 0 ? ws.data_ptr() : nullptr;
+  const int d = static_cast<int>(q.size(2));
+  if (fp8) {
+    check_status(dk_paged_attention_varlen_fp8(&p, dt, d, static_cast<int>(max_query_len), static_cast<int>(max_seq_len),
+                                               static_cast<float>(k_scale), static_cast<float>(v_scale), ws_ptr, ws_bytes,
+                                               stream_of(q)),
+                 op);
+  } else {
+    check_status(dk_paged_attention_varlen(&p, dt, d, static_cast<int>(max_query_len), static_cast<int>(max_seq_len),
+                                           ws_ptr, ws_bytes, stream_of(q)),
+                 op);
+  }
+}
+
+}  // namespace
+
+void paged_attention_varlen(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                            const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                            const at::Tensor& query_start_loc, double scale, int64_t max_query_len,
+                            int64_t max_seq_len, int64_t window, double softcap,
+                            const std::optional<at::Tensor>& alibi_slopes,
+                            const std::optional<at::Tensor>& prefix_lens) {
+  varlen_impl(out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len,
+              window, softcap, alibi_slopes, prefix_lens, false, 1.0, 1.0, "paged_attention_varlen");
+}
+
+void paged_attention_varlen_fp8(at::Tensor& out, const at::Tensor& q, const at::Tensor& k_cache,
+                                const at::Tensor& v_cache, const at::Tensor& block_tables, const at::Tensor& seq_lens,
+                                const at::Tensor& query_start_loc, double scale, int64_t max_query_len,
+                                int64_t max_seq_len, int64_t window, double softcap,
+                                const std::optional<at::Tensor>& alibi_slopes,
+                                const std::optional<at::Tensor>& prefix_lens, double k_scale, double v_scale) {
+  varlen_impl(out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len,
+              window, softcap, alibi_slopes, prefix_lens, true, k_scale, v_scale, "paged_attention_varlen_fp8");
+}
+
+// ---------------------------------------------------------------------------
 // Registration (csrc/ops.cu:270-286)
 // ---------------------------------------------------------------------------
 TORCH_LIBRARY(decode_kernels, m) {
@@ -621,6 +920,29 @@ TORCH_LIBRARY(decode_kernels, m) {
       "gemm_tn_rotary_embedding_and_cache_fp8(Tensor! qkv, Tensor a, Tensor b, Tensor? bias, Tensor positions, "
       "Tensor! query, Tensor! key, Tensor value, int head_size, Tensor cos_sin_cache, bool is_neox, "
       "Tensor! key_cache, Tensor! value_cache, Tensor slot_mapping, float k_scale, float v_scale) -> ()");
+  m.def(
+      "build_slot_mapping(Tensor query_start_loc, Tensor seq_lens, Tensor! block_tables, int block_size, "
+      "Tensor? free_blocks, Tensor! positions, Tensor! slot_mapping, Tensor!? num_new_blocks) -> ()");
+  m.def(
+      "qk_norm_rotary_embedding(Tensor positions, Tensor query, Tensor key, Tensor q_weight, Tensor k_weight, "
+      "float eps, int head_size, Tensor cos_sin_cache, bool is_neox, Tensor! query_out, Tensor! key_out) -> ()");
+  m.def(
+      "qk_norm_rotary_embedding_and_cache(Tensor positions, Tensor query, Tensor key, Tensor value, Tensor q_weight, "
+      "Tensor k_weight, float eps, int head_size, Tensor cos_sin_cache, bool is_neox, Tensor! key_cache, "
+      "Tensor! value_cache, Tensor slot_mapping, Tensor! query_out) -> ()");
+  m.def(
+      "qk_norm_rotary_embedding_and_cache_fp8(Tensor positions, Tensor query, Tensor key, Tensor value, "
+      "Tensor q_weight, Tensor k_weight, float eps, int head_size, Tensor cos_sin_cache, bool is_neox, "
+      "Tensor! key_cache, Tensor! value_cache, Tensor slot_mapping, Tensor! query_out, float k_scale, float v_scale) "
+      "-> ()");
+  m.def(
+      "paged_attention_varlen(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "
+      "Tensor seq_lens, Tensor query_start_loc, float scale, int max_query_len, int max_seq_len, int window, "
+      "float softcap, Tensor? alibi_slopes, Tensor? prefix_lens) -> ()");
+  m.def(
+      "paged_attention_varlen_fp8(Tensor! out, Tensor q, Tensor k_cache, Tensor v_cache, Tensor block_tables, "
+      "Tensor seq_lens, Tensor query_start_loc, float scale, int max_query_len, int max_seq_len, int window, "
+      "float softcap, Tensor? alibi_slopes, Tensor? prefix_lens, float k_scale, float v_scale) -> ()");
 }
 
 TORCH_LIBRARY_IMPL(decode_kernels, CUDA, m) {
@@ -638,6 +960,12 @@ TORCH_LIBRARY_IMPL(decode_kernels, CUDA, m) {
   m.impl("gemm_tn_add_rms_norm", &gemm_tn_add_rms_norm);
   m.impl("gemm_tn_rotary_embedding_and_cache", &gemm_tn_rotary_embedding_and_cache);
   m.impl("gemm_tn_rotary_embedding_and_cache_fp8", &gemm_tn_rotary_embedding_and_cache_fp8);
+  m.impl("build_slot_mapping", &build_slot_mapping);
+  m.impl("qk_norm_rotary_embedding", &qk_norm_rotary_embedding);
+  m.impl("qk_norm_rotary_embedding_and_cache", &qk_norm_rotary_embedding_and_cache);
+  m.impl("qk_norm_rotary_embedding_and_cache_fp8", &qk_norm_rotary_embedding_and_cache_fp8);
+  m.impl("paged_attention_varlen", &paged_attention_varlen);
+  m.impl("paged_attention_varlen_fp8", &paged_attention_varlen_fp8);
 }
 
 // Python module entry point: an empty module; importing it loads this

@@ -136,6 +136,47 @@ if _AVAILABLE:
               value_cache, slot_mapping, k_scale, v_scale):
             return None
 
+    if _has_op("build_slot_mapping"):
+
+        @torch.library.register_fake("decode_kernels::build_slot_mapping")
+        def _(query_start_loc, seq_lens, block_tables, block_size, free_blocks, positions, slot_mapping,
+              num_new_blocks):
+            return None
+
+    if _has_op("qk_norm_rotary_embedding"):
+
+        @torch.library.register_fake("decode_kernels::qk_norm_rotary_embedding")
+        def _(positions, query, key, q_weight, k_weight, eps, head_size, cos_sin_cache, is_neox, query_out, key_out):
+            return None
+
+    if _has_op("qk_norm_rotary_embedding_and_cache"):
+
+        @torch.library.register_fake("decode_kernels::qk_norm_rotary_embedding_and_cache")
+        def _(positions, query, key, value, q_weight, k_weight, eps, head_size, cos_sin_cache, is_neox, key_cache,
+              value_cache, slot_mapping, query_out):
+            return None
+
+    if _has_op("qk_norm_rotary_embedding_and_cache_fp8"):
+
+        @torch.library.register_fake("decode_kernels::qk_norm_rotary_embedding_and_cache_fp8")
+        def _(positions, query, key, value, q_weight, k_weight, eps, head_size, cos_sin_cache, is_neox, key_cache,
+              value_cache, slot_mapping, query_out, k_scale, v_scale):
+            return None
+
+    if _has_op("paged_attention_varlen"):
+
+        @torch.library.register_fake("decode_kernels::paged_attention_varlen")
+        def _(out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len,
+              window, softcap, alibi_slopes, prefix_lens):
+            return None
+
+    if _has_op("paged_attention_varlen_fp8"):
+
+        @torch.library.register_fake("decode_kernels::paged_attention_varlen_fp8")
+        def _(out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, scale, max_query_len, max_seq_len,
+              window, softcap, alibi_slopes, prefix_lens, k_scale, v_scale):
+            return None
+
 
 # ---------------------------------------------------------------------------
 # Paged attention
@@ -407,3 +448,179 @@ def gemm_rotary_embedding_and_cache(
             slot_mapping
         )
     return query, key, value
+
+
+# ---------------------------------------------------------------------------
+# The attention step of a ragged batch, whose sequences bring any number of new
+# tokens: one (decode), a few (speculation) or many (prompts and their chunks).
+# No counterparts in DecodeKernels.
+# ---------------------------------------------------------------------------
+def build_slot_mapping(
+    query_start_loc: torch.Tensor,
+    seq_lens: torch.Tensor,
+    block_tables: torch.Tensor,
+    block_size: int,
+    num_tokens: int,
+    free_blocks: torch.Tensor | None = None,
+    positions: torch.Tensor | None = None,
+    slot_mapping: torch.Tensor | None = None,
+    num_new_blocks: torch.Tensor | None = None,
+):
+    """Positions and cache slots of a ragged batch's tokens, on the GPU.
+
+    Sequence s brings tokens [query_start_loc[s], query_start_loc[s + 1]), the
+    last ones of its seq_lens[s]; the tokens before them are in the cache, in
+    the first blocks of block_tables[s]. The further blocks that its new tokens
+    need are taken from ``free_blocks`` (int32), in the order of the sequences,
+    and entered into ``block_tables`` in place; without ``free_blocks`` the
+    table must hold them already. All int32 on one device: query_start_loc
+    [num_seqs + 1] from 0 and non-decreasing, seq_lens [num_seqs], block_tables
+    [num_seqs, max_blocks].
+
+    Returns (positions, slot_mapping, num_new_blocks): int64 [num_tokens] each,
+    as ``qk_norm_rotary_embedding_and_cache`` and ``reshape_and_cache`` take
+    them, and int32 [1], how many blocks the new tokens need beyond those held.
+    Tokens behind the last sequence (a padded batch) get position and slot -1;
+    a token without a block (table or free list too short, a negative entry)
+    gets slot -1, which the cache writes skip. Outputs may be given."""
+    _require()
+    dev = query_start_loc.device
+    if positions is None:
+        positions = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    if slot_mapping is None:
+        slot_mapping = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    if num_new_blocks is None:
+        num_new_blocks = torch.empty(1, dtype=torch.int32, device=dev)
+    if positions.shape[0] != num_tokens:
+        raise ValueError(f"positions must have num_tokens = {num_tokens} entries, got {positions.shape[0]}")
+    torch.ops.decode_kernels.build_slot_mapping(
+        query_start_loc, seq_lens, block_tables, int(block_size), free_blocks, positions, slot_mapping, num_new_blocks
+    )
+    return positions, slot_mapping, num_new_blocks
+
+
+def qk_norm_rotary_embedding(
+    positions: torch.Tensor,
+    query: torch.Tensor,
+    key: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    eps: float,
+    head_size: int,
+    cos_sin_cache: torch.Tensor,
+    is_neox: bool = True,
+    query_out: torch.Tensor | None = None,
+    key_out: torch.Tensor | None = None,
+):
+    """RMS norm of every query and key head (``q_weight`` / ``k_weight``
+    [head_size]), then ``rotary_embedding``, in one pass with one rounding; in
+    place unless ``query_out`` / ``key_out`` are given. A token whose position
+    lies outside ``cos_sin_cache`` is padding: its rows are not written.
+    Returns (query_out, key_out)."""
+    _require()
+    query_out = query if query_out is None else query_out
+    key_out = key if key_out is None else key_out
+    torch.ops.decode_kernels.qk_norm_rotary_embedding(
+        positions, query, key, q_weight, k_weight, float(eps), int(head_size), cos_sin_cache, bool(is_neox), query_out,
+        key_out
+    )
+    return query_out, key_out
+
+
+def qk_norm_rotary_embedding_and_cache(
+    positions: torch.Tensor,
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    q_weight: torch.Tensor,
+    k_weight: torch.Tensor,
+    eps: float,
+    head_size: int,
+    cos_sin_cache: torch.Tensor,
+    is_neox: bool,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+    query_out: torch.Tensor | None = None,
+):
+    """``qk_norm_rotary_embedding`` with the cache write: the query is normed
+    and rotated (in place unless ``query_out`` is given), the normed and rotated
+    key and the value go to the cache slots (also ``torch.float8_e4m3fn`` caches
+    with k_scale / v_scale). ``key`` itself is only read. Padding tokens
+    (positions outside the table) are left out of the cache too; negative slots
+    are skipped. Returns query_out."""
+    _require()
+    query_out = query if query_out is None else query_out
+    if key_cache.dtype == torch.float8_e4m3fn:
+        torch.ops.decode_kernels.qk_norm_rotary_embedding_and_cache_fp8(
+            positions, query, key, value, q_weight, k_weight, float(eps), int(head_size), cos_sin_cache, bool(is_neox),
+            key_cache, value_cache, slot_mapping, query_out, float(k_scale), float(v_scale)
+        )
+        return query_out
+    if k_scale != 1.0 or v_scale != 1.0:
+        raise ValueError("k_scale / v_scale apply to an fp8 (float8_e4m3fn) KV cache only")
+    torch.ops.decode_kernels.qk_norm_rotary_embedding_and_cache(
+        positions, query, key, value, q_weight, k_weight, float(eps), int(head_size), cos_sin_cache, bool(is_neox),
+        key_cache, value_cache, slot_mapping, query_out
+    )
+    return query_out
+
+
+def paged_attention_varlen(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    scale: float | None = None,
+    max_query_len: int | None = None,
+    max_seq_len: int | None = None,
+    window: int = 0,
+    softcap: float = 0.0,
+    alibi_slopes: torch.Tensor | None = None,
+    prefix_lens: torch.Tensor | None = None,
+    out: torch.Tensor | None = None,
+    k_scale: float = 1.0,
+    v_scale: float = 1.0,
+) -> torch.Tensor:
+    """Attention of a ragged batch's new tokens over a paged KV cache that
+    holds their own keys and values already.
+
+    q: [num_tokens, num_q_heads, head_dim]; sequence s brings its rows
+    [query_start_loc[s], query_start_loc[s + 1]), the last ones of its
+    seq_lens[s] tokens. Caches and block_tables as ``paged_attention_decode``
+    (rows 16-byte aligned; also ``torch.float8_e4m3fn`` with k_scale / v_scale).
+    The token at position i sees key j <= i, with ``window`` > 0 only those
+    with j > i - window, and every key below prefix_lens[s] (int32, optional).
+    Scores are scale * q.k, capped to softcap * tanh(. / softcap) with
+    ``softcap`` > 0, less alibi_slopes[h] * |i - j| (float32, optional). A token
+    that sees no key gives zeros; rows behind the last sequence are not written.
+
+    ``max_query_len`` / ``max_seq_len`` must bound the new tokens and the
+    lengths of every sequence; passing them avoids a device-to-host sync."""
+    _require()
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    num_seqs = query_start_loc.shape[0] - 1
+    if max_query_len is None:
+        max_query_len = int((query_start_loc[1:] - query_start_loc[:-1]).max().item()) if num_seqs > 0 else 0
+    if max_seq_len is None:
+        max_seq_len = int(seq_lens[:num_seqs].max().item()) if num_seqs > 0 else 0
+    if out is None:
+        out = torch.empty_like(q)
+    if k_cache.dtype == torch.float8_e4m3fn:
+        torch.ops.decode_kernels.paged_attention_varlen_fp8(
+            out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, float(scale), int(max_query_len),
+            int(max_seq_len), int(window), float(softcap), alibi_slopes, prefix_lens, float(k_scale), float(v_scale)
+        )
+        return out
+    if k_scale != 1.0 or v_scale != 1.0:
+        raise ValueError("k_scale / v_scale apply to an fp8 (float8_e4m3fn) KV cache only")
+    torch.ops.decode_kernels.paged_attention_varlen(
+        out, q, k_cache, v_cache, block_tables, seq_lens, query_start_loc, float(scale), int(max_query_len),
+        int(max_seq_len), int(window), float(softcap), alibi_slopes, prefix_lens
+    )
+    return out

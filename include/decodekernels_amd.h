@@ -339,6 +339,138 @@ int dk_gemm_tn_rotary_embedding_and_cache_fp8(int dtype, const void* A, const vo
                                               float k_scale, float v_scale, void* workspace, int64_t workspace_bytes,
                                               void* stream);
 
+/*
+ * Positions, cache slots and new cache blocks of a ragged batch's tokens, on
+ * the GPU. Sequence s brings tokens [query_start_loc[s], query_start_loc[s+1]),
+ * n_s of them, the last ones of its seq_lens[s]; the c_s = seq_lens[s] - n_s
+ * before them are in the cache, in the first ceil(c_s / block_size) blocks of
+ * its block-table row. The blocks that its new tokens need beyond those are
+ * taken from free_blocks, in the order of the sequences, and entered into
+ * block_tables; *num_new_blocks (may be NULL) is how many all sequences need.
+ *   positions[t]    = c_s + t - query_start_loc[s]
+ *   slot_mapping[t] = block * block_size + positions[t] % block_size
+ * with block = the sequence's block positions[t] / block_size. free_blocks may
+ * be NULL: block_tables then holds the new blocks already (and is only read).
+ *   query_start_loc [num_seqs + 1] int32, non-decreasing, from 0
+ *   seq_lens        [num_seqs] int32
+ *   block_tables    [num_seqs, max_blocks] int32, row stride bt_stride
+ *   free_blocks     [num_free_blocks] int32
+ *   positions, slot_mapping  [num_tokens] int64
+ * Tokens behind the last sequence get -1 / -1. A token whose block is past the
+ * table's columns, past the free list or a negative entry gets slot -1, and
+ * one that its sequence's length leaves no place gets -1 / -1:
+ * dk_reshape_and_cache and dk_qk_norm_rotary_embedding_and_cache skip it.
+ * No counterpart in DecodeKernels, which leaves this step to the serving engine.
+ */
+typedef struct dk_slot_mapping_params {
+  const int32_t* query_start_loc;
+  const int32_t* seq_lens;
+  int32_t* block_tables;
+  const int32_t* free_blocks;
+  int64_t* positions;
+  int64_t* slot_mapping;
+  int32_t* num_new_blocks;
+  int64_t bt_stride;
+  int32_t num_seqs, num_tokens, block_size, max_blocks, num_free_blocks;
+} dk_slot_mapping_params;
+
+int dk_build_slot_mapping(const dk_slot_mapping_params* p, void* stream);
+
+/*
+ * RMS norm of every query and key head (over head_size, one weight vector each
+ * for queries and keys), then the rotation of dk_rotary_embedding, in fp32 with
+ * one rounding at the end: query -> query_out, key -> key_out. The outputs may
+ * be the inputs themselves (same pointer and strides), not overlap them
+ * otherwise. A token whose position lies outside the table is padding: its
+ * rows are left as they were.
+ *   q_weight, k_weight  [head_size] (dtype)
+ * No counterpart in DecodeKernels.
+ */
+typedef struct dk_qk_norm_params {
+  const void* q_weight;
+  const void* k_weight;
+  void* query_out;
+  void* key_out;
+  int64_t qo_stride_token, qo_stride_head;
+  int64_t ko_stride_token, ko_stride_head;
+  float eps;
+} dk_qk_norm_params;
+
+int dk_qk_norm_rotary_embedding(const dk_rotary_params* r, const dk_qk_norm_params* n, int dtype, void* stream);
+
+/*
+ * The same with the cache write: the normed and rotated key and the value go
+ * to the cache slots of c as by dk_reshape_and_cache (negative slots and slots
+ * past the cache are skipped; the query is written all the same), or quantized
+ * into e4m3fn caches (_fp8; from fp32, without a rounding to dtype between).
+ * The key itself is only read and n->key_out is ignored. r->key must be c->key
+ * with the same strides.
+ * No counterpart in DecodeKernels.
+ */
+int dk_qk_norm_rotary_embedding_and_cache(const dk_rotary_params* r, const dk_qk_norm_params* n,
+                                          const dk_cache_write_params* c, int dtype, void* stream);
+int dk_qk_norm_rotary_embedding_and_cache_fp8(const dk_rotary_params* r, const dk_qk_norm_params* n,
+                                              const dk_cache_write_params* c, int dtype, float k_scale, float v_scale,
+                                              void* stream);
+
+/*
+ * Attention of a ragged batch's new tokens over the paged cache, in which
+ * their own keys and values are already. Sequence s brings query tokens
+ * [query_start_loc[s], query_start_loc[s+1]), the last ones of its seq_lens[s]
+ * tokens: one (decode), some (speculation) or many (a prompt or a chunk of it).
+ * The token at position i sees key j where j <= i and j > i - window (window 0:
+ * every j <= i), or where j < prefix_lens[s]; its scores are
+ *   x = scale * q . k,  x = softcap * tanh(x / softcap) (softcap 0: as it is),
+ *   x - alibi_slopes[h] * |i - j|
+ * and out is the softmax-weighted sum of the values it sees, zeros where it
+ * sees none. Rows of tokens behind the last sequence are not written. Keys and
+ * values that a token does not see have no influence on it, whatever they
+ * hold; block-table entries of blocks that no token sees are not used.
+ *   out, q        [num_tokens, num_q_heads, head_dim] (dtype), any token / head
+ *                 strides
+ *   k/v_cache, block_tables, seq_lens  as dk_paged_attn_params, with pointers
+ *                 and strides of the caches multiples of 16 bytes; max_blocks
+ *                 columns in block_tables
+ *   query_start_loc [num_seqs + 1] int32, non-decreasing, from 0
+ *   prefix_lens   [num_seqs] int32 or NULL
+ *   alibi_slopes  [num_q_heads] fp32 or NULL
+ * max_query_len and max_seq_len bound the new tokens and the lengths of every
+ * sequence. head_dim in {64, 96, 128, 192, 256} (fp8 caches: not 96), at most
+ * DK_MAX_GQA_GROUP query heads per KV head.
+ * workspace (16-byte aligned) of dk_paged_attention_varlen_workspace_bytes
+ * bytes lets the keys of a token be split over workgroups, whose fp32 partial
+ * results a second kernel joins in a fixed order; NULL or a smaller one: not
+ * split. It must not be shared by calls that run concurrently.
+ * No counterpart in DecodeKernels, whose attention takes one token per sequence
+ * and plain scores (csrc/paged_attention.cuh:73-333).
+ */
+typedef struct dk_varlen_attn_params {
+  void* out;
+  const void* q;
+  const void* k_cache;
+  const void* v_cache;
+  const int32_t* block_tables;
+  const int32_t* seq_lens;
+  const int32_t* query_start_loc;
+  const int32_t* prefix_lens;
+  const float* alibi_slopes;
+  int64_t q_stride_token, q_stride_head;
+  int64_t out_stride_token, out_stride_head;
+  int64_t k_stride_block, k_stride_token, k_stride_head;
+  int64_t v_stride_block, v_stride_token, v_stride_head;
+  int64_t bt_stride;
+  int32_t num_tokens, num_seqs, num_q_heads, num_kv_heads, block_size, num_blocks, max_blocks, window;
+  float scale, softcap;
+} dk_varlen_attn_params;
+
+int64_t dk_paged_attention_varlen_workspace_bytes(const dk_varlen_attn_params* p, int head_dim, int max_query_len,
+                                                  int max_seq_len);
+int dk_paged_attention_varlen(const dk_varlen_attn_params* p, int dtype, int head_dim, int max_query_len,
+                              int max_seq_len, void* workspace, int64_t workspace_bytes, void* stream);
+int dk_paged_attention_varlen_fp8(const dk_varlen_attn_params* p, int dtype, int head_dim, int max_query_len,
+                                  int max_seq_len, float k_scale, float v_scale, void* workspace,
+                                  int64_t workspace_bytes, void* stream);
+
 /* Description of the last argument error raised on this thread ("" if none).
  * The reference reports these through TORCH_CHECK messages (csrc/ops.cu). */
 const char* dk_last_error(void);

@@ -38,27 +38,22 @@ struct KParams {
   int num_tokens, num_seqs, hq, group, block_size, num_blocks;
   int max_len;             // no length goes past it: the caller's bound, and what the tables can hold
   int window;              // keys a token sees, itself included; max_len where it sees all before it
-  int hkv, rows_short;     // sequences of more than rows_short rows a KV head run in tiles (tile_kernel)
-  int split_items;         // workgroups that the tiles of a call may be split over; 0: never split
-  float* ws;               // partial results
+  int hkv;
+  int split_items;         // tile_kernel: workgroups that the tiles of a call may be split over; 0: never split
+  int shares;              // row_kernel: workgroups a KV head, of equal shares of all key tiles; 0: one a sequence
+  int slot_rows;           // row_kernel: rows of a slot
+  float* ws;               // partial results: sums, row by row of a slot
+  float* ws_ml;            // their reference maximum (log2 units) and exp-sum
+  int32_t* ws_first;       // row_kernel: a sequence's first workgroup, and how many
   uint32_t bs_mul;         // j / block_size = (j * bs_mul) >> bs_shift, for j < 2^31
   int bs_shift;
-  float scale, softcap, k_scale, v_scale;
-  // In log2 units: the factor of q.k (positive: its sign goes to q), the cap
-  // and, for its tanh, exp(2 y) = 2^(cap_in s).
-  float scale2, cap2, cap_in;
+  float v_scale;           // of an fp8 cache (1 otherwise)
+  // In log2 units: the cap (0: none) and the positive factor of q.k, whose sign
+  // goes to q: the score's, or with a cap that of the exponent of e^(2 y) in
+  // tanh y = 1 - 2 / (e^(2 y) + 1).
+  float cap2, scale2;
   uint32_t q_sign;
 };
-
-// The sequence that owns token t: how many end at or before it (num_seqs: none
-// does). The lanes count side by side.
-__device__ __forceinline__ int find_seq(const KParams& p, int t, int lane) {
-  int s = 0;
-  for (int i = lane; i < p.num_seqs; i += kWave) s += p.starts[i + 1] <= t ? 1 : 0;
-#pragma unroll
-  for (int off = kWave / 2; off > 0; off >>= 1) s += __shfl_xor(s, off, kWave);
-  return s;
-}
 
 // 8 e4m3fn bytes as 8 elements of E, exactly.
 template <typename E>
@@ -69,84 +64,6 @@ __device__ __forceinline__ u32x4 fp8x8_to(u32x2 w) {
   const auto d = __builtin_amdgcn_cvt_pk_f32_fp8(w[1], true);
   return u32x4{pack2<E>(a[0], a[1]), pack2<E>(b[0], b[1]), pack2<E>(c[0], c[1]), pack2<E>(d[0], d[1])};
 }
-
-template <typename E, bool FP8>
-__device__ __forceinline__ float element(const void* base, int64_t i) {
-  if constexpr (FP8) {
-    return __builtin_amdgcn_cvt_f32_fp8(static_cast<const uint8_t*>(base)[i], 0);
-  } else {
-    return E::to_float(static_cast<const uint16_t*>(base)[i]);
-  }
-}
-
-// One wave per (token, query head): scores of 64 keys at a time, a key per
-// lane, then the weighted sum with the columns over the lanes.
-template <typename E, bool FP8>
-__global__ __launch_bounds__(kWave) void simple_kernel(const KParams p, int d) {
-  __shared__ float q[256];
-  __shared__ float weight[kWave];
-  const int lane = threadIdx.x;
-  const int t = blockIdx.x / p.hq;
-  const int h = blockIdx.x - t * p.hq;
-  const int kvh = h / p.group;
-  const int s = find_seq(p, t, lane);
-  if (s >= p.num_seqs) return;  // a row behind the last sequence
-  const int first = max(p.starts[s], 0);
-  const int n = min(p.starts[s + 1], p.num_tokens) - first;
-  const int len = max(min(p.lens[s], p.max_len), 0);
-  const int pos = len - n + (t - first);
-  if (static_cast<int64_t>(n) * p.group > p.rows_short) return;
-  const int pre = p.prefix != nullptr ? min(max(p.prefix[s], 0), len) : 0;
-  for (int i = lane; i < d; i += kWave) q[i] = E::to_float(p.q[static_cast<int64_t>(t) * p.q_st + static_cast<int64_t>(h) * p.q_sh + i]);
-  __syncthreads();
-  const float slope = p.slopes != nullptr ? p.slopes[h] : 0.0f;
-  float top = -__builtin_huge_valf(), total = 0.0f;
-  float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  const int low = max(pos - p.window + 1, 0);
-  const int end = max(pre, pos + 1);
-  for (int j0 = 0; j0 < end; j0 += kWave) {
-    if (j0 >= pre && j0 + kWave <= low) continue;
-    const int j = j0 + lane;
-    const bool sees = j < pre || (j <= pos && j >= low);
-    float x = -__builtin_huge_valf();
-    int64_t at = 0;
-    if (sees) {
-      const int64_t page = min(max(p.tables[static_cast<int64_t>(s) * p.bt_stride + j / p.block_size], 0), p.num_blocks - 1);
-      const int64_t off = j % p.block_size;
-      const int64_t row = page * p.k_sb + off * p.k_st + static_cast<int64_t>(kvh) * p.k_sh;
-      at = page * p.v_sb + off * p.v_st + static_cast<int64_t>(kvh) * p.v_sh;
-      float dot = 0.0f;
-      for (int i = 0; i < d; ++i) dot += q[i] * element<E, FP8>(p.k, row + i);
-      x = dot * p.scale * p.k_scale;
-      if (p.softcap > 0.0f) x = p.softcap * tanhf(x / p.softcap);
-      x -= slope * static_cast<float>(pos > j ? pos - j : j - pos);
-    }
-    const float new_top = fmaxf(top, wave_max(x));
-    const float ref = new_top == -__builtin_huge_valf() ? 0.0f : new_top;
-    const float w = sees ? __builtin_amdgcn_exp2f((x - ref) * kLog2e) : 0.0f;
-    const float alpha = __builtin_amdgcn_exp2f((top - ref) * kLog2e);
-    total = total * alpha + wave_sum(w);
-    top = new_top;
-    __syncthreads();
-    weight[lane] = w;
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 4; ++c) acc[c] *= alpha;
-    const uint64_t seen = __ballot(sees);
-    for (int jj = 0; jj < kWave; ++jj) {
-      if (!((seen >> jj) & 1)) continue;  // never a product with a hidden value
-      const int64_t row = __shfl(at, jj, kWave);
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-        if (lane + c * kWave < d) acc[c] += weight[jj] * element<E, FP8>(p.v, row + lane + c * kWave);
-    }
-  }
-  uint16_t* out = p.out + static_cast<int64_t>(t) * p.o_st + static_cast<int64_t>(h) * p.o_sh;
-#pragma unroll
-  for (int c = 0; c < 4; ++c)
-    if (lane + c * kWave < d) out[lane + c * kWave] = E::from_float(total == 0.0f ? 0.0f : acc[c] / total * p.v_scale);
-}
-
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -161,11 +78,16 @@ __device__ __forceinline__ f32x16 mfma_32x32x16<F16>(u32x4 a, u32x4 b, f32x16 c)
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
+// Rows of a KV head, (token, query head of its group) pairs, up to which a
+// sequence runs in row_kernel, which has one 16-column MFMA operand for them.
+constexpr int kShortRows = 16;
 constexpr int kTileWaves = 4;
 constexpr int kTileThreads = kTileWaves * kWave;
 constexpr int kTileRows = 32 * kTileWaves;  // (token, query head of the group) rows of a workgroup
 constexpr int kRsrcWord3 = 0x00020000;      // word 3 of a gfx9-family buffer resource for raw loads
 constexpr int kSeqsPerThread = 4;
+constexpr int kWholeKeys = 512;             // keys up to which a sequence of few rows is never cut
+constexpr int kMinShare = 16;               // key tiles a workgroup of row_kernel takes at least
 
 // Infinities and NaN of the dtype: the exponent bits of an element, and the
 // lowest of them.
@@ -219,12 +141,23 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// The kernel's arguments, to be loaded where they are used: an argument that
+// the compiler sees only here does not stay in scalar registers around it.
+// KParams is the one parameter, at the start of the argument segment.
+typedef const __attribute__((address_space(4))) KParams Args;
+__device__ __forceinline__ Args& fresh_args() {
+  auto a = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
+  __asm__ volatile("" : "+s"(a));
+  return *a;
+}
+
 // A uniform int32 through the scalar cache (data of earlier kernels only).
 __device__ __forceinline__ int scalar_load(const int32_t* base, int64_t i) {
   return ((const __attribute__((address_space(4))) int32_t*)base)[i];
 }
 
-__device__ __forceinline__ int div_block(const KParams& p, int j) {
+template <typename Params>
+__device__ __forceinline__ int div_block(const Params& p, int j) {
   return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(j)) * p.bs_mul) >> p.bs_shift);
 }
 
@@ -233,7 +166,8 @@ struct Seq {
   int first, n, len, pre;
 };
 
-__device__ __forceinline__ Seq make_seq(const KParams& p, int start, int end, int len, int pre) {
+template <typename Params>
+__device__ __forceinline__ Seq make_seq(const Params& p, int start, int end, int len, int pre) {
   Seq q;
   q.first = min(max(start, 0), p.num_tokens);
   q.n = max(min(end, p.num_tokens) - q.first, 0);
@@ -247,56 +181,87 @@ struct LocateSmem {
   int seq, local;
 };
 
-// Row tiles of a sequence: none where its few rows run in the other kernel.
+// 4 columns of an output row, rounded; in one store where rows are 8-byte aligned.
+template <typename E, typename Params>
+__device__ __forceinline__ void store4(const Params& p, uint16_t* dst, f32x4 y) {
+  if ((reinterpret_cast<uintptr_t>(p.out) % 8 == 0) && p.o_st % 4 == 0 && p.o_sh % 4 == 0) {
+    *reinterpret_cast<u32x2*>(dst) = u32x2{pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) dst[i] = E::from_float(y[i]);
+  }
+}
+
+// Row tiles of a sequence: none where its few rows run in row_kernel.
 __device__ __forceinline__ int row_tiles(const KParams& p, int start, int end) {
   const int first = min(max(start, 0), p.num_tokens);
   const int64_t rows = static_cast<int64_t>(max(min(end, p.num_tokens) - first, 0)) * p.group;
-  return rows > p.rows_short ? static_cast<int>((rows + kTileRows - 1) / kTileRows) : 0;
+  return rows > kShortRows ? static_cast<int>((rows + kTileRows - 1) / kTileRows) : 0;
 }
 
-// The sequence and its tile that hold tile `target` of all, and the number of
-// tiles in all; seq = -1 past it. The whole workgroup counts, 4 sequences a
-// thread and step.
-__device__ __forceinline__ int locate_tile(const KParams& p, int target, LocateSmem& sm, int& seq, int& local) {
+// Sequences s0 .. s0 + 1023, 4 a thread: weight(s) units each. Sets w and the
+// units before each of them (from `base` on) and returns the units in all.
+template <typename Weight>
+__device__ __forceinline__ int scan_sequences(int num_seqs, int s0, int base, LocateSmem& sm, Weight weight,
+                                              int (&w)[kSeqsPerThread], int (&before)[kSeqsPerThread]) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  if (tid == 0) sm.seq = -1;
-  int base = 0;
-  for (int s0 = 0; s0 < p.num_seqs; s0 += kTileThreads * kSeqsPerThread) {
-    int st[kSeqsPerThread + 1], w[kSeqsPerThread], sum = 0;
-    const int s = s0 + tid * kSeqsPerThread;
+  const int s = s0 + tid * kSeqsPerThread;
+  int sum = 0;
 #pragma unroll
-    for (int i = 0; i <= kSeqsPerThread; ++i) st[i] = p.starts[min(s + i, p.num_seqs)];
-#pragma unroll
-    for (int i = 0; i < kSeqsPerThread; ++i) {
-      w[i] = s + i < p.num_seqs ? row_tiles(p, st[i], st[i + 1]) : 0;
-      sum += w[i];
-    }
-    int scan = sum;
-#pragma unroll
-    for (int off = 1; off < kWave; off <<= 1) {
-      const int v = __shfl_up(scan, off, kWave);
-      if (lane >= off) scan += v;
-    }
-    if (lane == kWave - 1) sm.wave_total[wave] = scan;
-    lds_barrier();
-    int before = base + scan - sum;
-    for (int i = 0; i < kTileWaves; ++i) {
-      if (i < wave) before += sm.wave_total[i];
-      base += sm.wave_total[i];
-    }
-#pragma unroll
-    for (int i = 0; i < kSeqsPerThread; ++i) {
-      if (target >= before && target < before + w[i]) {
-        sm.seq = s + i;
-        sm.local = target - before;
-      }
-      before += w[i];
-    }
-    lds_barrier();
+  for (int i = 0; i < kSeqsPerThread; ++i) {
+    w[i] = s + i < num_seqs ? weight(s + i) : 0;
+    sum += w[i];
   }
+  int scan = sum;
+#pragma unroll
+  for (int off = 1; off < kWave; off <<= 1) {
+    const int v = __shfl_up(scan, off, kWave);
+    if (lane >= off) scan += v;
+  }
+  lds_barrier();  // the last scan's totals and find have been read
+  if (lane == kWave - 1) sm.wave_total[wave] = scan;
+  if (tid == 0) sm.seq = -1;
+  lds_barrier();
+  int at = base + scan - sum, total = 0;
+#pragma unroll
+  for (int i = 0; i < kTileWaves; ++i) {
+    if (i < wave) at += sm.wave_total[i];
+    total += sm.wave_total[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kSeqsPerThread; ++i) {
+    before[i] = at;
+    at += w[i];
+  }
+  return __builtin_amdgcn_readfirstlane(total);
+}
+
+// Units of all sequences; then, with target(total), the sequence and the unit
+// of it that hold this one of them (seq = -1: it is past them).
+template <typename Weight, typename Target>
+__device__ __forceinline__ int locate(int num_seqs, LocateSmem& sm, Weight weight, Target target, int& seq, int& local) {
+  constexpr int kStep = kTileThreads * kSeqsPerThread;
+  const int last = (num_seqs - 1) / kStep * kStep;
+  int w[kSeqsPerThread], before[kSeqsPerThread];
+  int total = 0;
+  for (int s0 = 0; s0 < num_seqs; s0 += kStep) total += scan_sequences(num_seqs, s0, total, sm, weight, w, before);
+  const int want = target(total);
+  int base = 0;
+  for (int s0 = last > 0 ? 0 : last; s0 < num_seqs; s0 += kStep) {
+    if (last > 0) base += scan_sequences(num_seqs, s0, base, sm, weight, w, before);  // else w and before still hold
+#pragma unroll
+    for (int i = 0; i < kSeqsPerThread; ++i) {
+      if (want >= before[i] && want < before[i] + w[i]) {
+        sm.seq = s0 + static_cast<int>(threadIdx.x) * kSeqsPerThread + i;
+        sm.local = want - before[i];
+      }
+    }
+    if (last > 0 && want < base) break;
+  }
+  lds_barrier();
   seq = __builtin_amdgcn_readfirstlane(sm.seq);
   local = __builtin_amdgcn_readfirstlane(sm.local);
-  return base;
+  return total;
 }
 
 // The key tiles that some row of a workgroup sees: those of the prefix, then
@@ -362,21 +327,18 @@ void tile_kernel(const KParams p) {
   // Later tiles (long ones under a causal mask) first; the KV heads of a tile
   // next to one another, so that with 8 of them each XCD's L2 holds one head.
   const int item = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);
-  int seq, local, parts = 1, part = 0, kv_head, total;
-  if (p.split_items == 0) {
-    kv_head = p.hkv - 1 - item % p.hkv;
-    total = locate_tile(p, item / p.hkv, loc, seq, local);
-  } else {
-    // Few tiles: each over as many workgroups as make split_items in all. How
-    // many tiles there are is known only now.
-    total = locate_tile(p, -1, loc, seq, local);
-    if (total == 0) return;
-    parts = max(p.split_items / (total * p.hkv), 1);
-    kv_head = p.hkv - 1 - item % p.hkv;
-    part = (item / p.hkv) % parts;
-    lds_barrier();
-    locate_tile(p, item / p.hkv / parts, loc, seq, local);
-  }
+  const int kv_head = p.hkv - 1 - item % p.hkv;
+  // With few tiles each goes over as many workgroups as make split_items in
+  // all; how many tiles there are is known only now.
+  int seq, local, parts = 1;
+  locate(
+      p.num_seqs, loc, [&](int s) { return row_tiles(p, p.starts[s], p.starts[s + 1]); },
+      [&](int total) {
+        if (p.split_items > 0 && total > 0) parts = max(p.split_items / (total * p.hkv), 1);
+        return item / p.hkv / parts;
+      },
+      seq, local);
+  const int part = item / p.hkv % parts;
   if (seq < 0) return;
   const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), scalar_load(p.lens, seq),
                           p.prefix != nullptr ? scalar_load(p.prefix, seq) : 0);
@@ -536,14 +498,14 @@ void tile_kernel(const KParams p) {
       }
     }
     float factor = p.scale2;
-    if (p.softcap > 0.0f) {
+    if (p.cap2 > 0.0f) {
       // tanh y = 1 - 2 / (e^(2y) + 1): -1 and 1 at the ends, absolute error of
       // an fp32 step of 1 near 0.
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-          s[b][i] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][i] * p.cap_in) + 1.0f);
+          s[b][i] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][i] * p.scale2) + 1.0f);
       factor = 1.0f;
     }
     if (p.slopes != nullptr) {
@@ -678,78 +640,594 @@ void tile_kernel(const KParams p) {
   if (32 * wave + l32 >= rows) return;
   if (parts > 1) {
     // Partial results: sums against m_ref, joined by tile_join_kernel.
-    const int64_t slot = ((static_cast<int64_t>(item / p.hkv / parts) * p.hkv + kv_head) * parts + part) * kTileRows +
-                         32 * wave + l32;
-    float* dst = p.ws + slot * (D + 2);
+    const int64_t slot = (static_cast<int64_t>(item) * kTileRows) + 32 * wave + l32;
+    float* dst = p.ws + slot * D;
     if (half == 0) {
-      dst[D] = m_ref;
-      dst[D + 1] = l_run;
+      p.ws_ml[2 * slot] = m_ref;
+      p.ws_ml[2 * slot + 1] = l_run;
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) dst[32 * b + 8 * (i / 4) + 4 * half + i % 4] = acc[b][i];
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(dst + 32 * b + 8 * g + 4 * half) =
+            f32x4{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
     return;
   }
   const float inv = l_run == 0.0f ? 0.0f : p.v_scale / l_run;
   uint16_t* dst = p.out + token * p.o_st + static_cast<int64_t>(q_head) * p.o_sh + 4 * half;
-  const bool wide = (reinterpret_cast<uintptr_t>(p.out) % 8 == 0) && p.o_st % 4 == 0 && p.o_sh % 4 == 0;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = l_run == 0.0f ? 0.0f : acc[b][4 * g + i] * inv;
-      if (wide) {
-        *reinterpret_cast<u32x2*>(dst + 32 * b + 8 * g) = u32x2{pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3])};
-      } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) dst[32 * b + 8 * g + i] = E::from_float(y[i]);
-      }
+      const f32x4 y = {acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
+      store4<E>(p, dst + 32 * b + 8 * g, l_run == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : y * inv);
     }
 }
 
+
+// LDS of row_kernel: each wave's current key tile, then, at the end of a piece,
+// the waves' sums in the same place.
+template <int D, bool FP8>
+struct RowSmem {
+  static constexpr int TT = FP8 ? 32 : 16;  // keys of a tile: as many bytes in flight with either cache
+  static constexpr int P = D + 16;          // row pitch, elements: 4 rows on distinct banks for the transpose reads
+  static constexpr int OP = D + 4;          // row pitch, floats
+  struct __attribute__((aligned(16))) Tile {
+    uint16_t k[TT * P];
+    uint16_t v[TT * P];
+    uint32_t up[TT][D / 32], down[TT][D / 32];  // as in TileSmem
+  };
+  union {
+    Tile tile[kTileWaves];
+    float o[kTileWaves][kShortRows * OP];
+  };
+  float m[kTileWaves][kShortRows], l[kTileWaves][kShortRows];
+  LocateSmem loc;
+};
+
+template <int D, bool FP8>
+constexpr int row_occupancy() {  // waves per SIMD
+  return D <= 64 ? 3 : D <= 128 ? 2 : 1;
+}
+
+// Decode and speculation: up to 16 rows a KV head. Bound by the reading of the
+// cache, so all rows take each key tile once, a wave streams whole rows of its
+// own tiles (two in flight in registers) and the work is cut over the cache's
+// length: with `shares`, workgroup g of a KV head takes the g-th of equal
+// shares of all sequences' key tiles, whatever their lengths. A piece that is
+// not a whole sequence leaves its sums in slot g + s (sequence s; no two pieces
+// share one) for row_join_kernel. Scores are S^T = K Q^T and the output O^T =
+// V^T P^T on 16x16 MFMAs: lane l holds row l % 16 of both.
+template <typename E, int D, bool FP8, bool BS16>
+__global__ __launch_bounds__(kTileThreads)
+__attribute__((amdgpu_waves_per_eu(row_occupancy<D, FP8>(), row_occupancy<D, FP8>())))
+void row_kernel(const KParams p) {
+  using Smem = RowSmem<D, FP8>;
+  constexpr int TT = Smem::TT, P = Smem::P, OP = Smem::OP;
+  constexpr int TG = TT / 16;           // 16-key groups of a tile: each lies in one cache block (BS16)
+  constexpr int CH = D / 32, NB = D / 16;
+  constexpr int ELT = FP8 ? 1 : 2;
+  constexpr int RB = D * ELT;           // bytes of a K (or V) row
+  constexpr int NI = 16 * RB / 1024;    // 16-byte loads of a lane for a group of K (or V)
+  constexpr int DEPTH = 2;
+  __shared__ Smem sm;
+  const int tid = threadIdx.x;
+  const int lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int l16 = lane % 16, lg = lane / 16;
+  const int kv_head = static_cast<int>(blockIdx.x) % p.hkv;
+  const int g = static_cast<int>(blockIdx.x) / p.hkv;
+
+  struct Work {
+    Seq sq;
+    int rows, pos0, lo;
+    KeyTiles tiles;
+  };
+  auto work_of = [&](const Seq& sq) {
+    Work w;
+    w.sq = sq;
+    const int64_t rows = static_cast<int64_t>(sq.n) * p.group;
+    // (slot_rows: no more than the caller's bound on the new tokens allows.)
+    w.rows = rows <= kShortRows ? min(static_cast<int>(rows), fresh_args().slot_rows) : 0;
+    w.pos0 = sq.len - sq.n;
+    w.lo = max(w.pos0 - p.window + 1, 0);
+    w.tiles = key_tiles<TT>(sq.pre, w.lo, sq.len);
+    return w;
+  };
+  // A sequence of any rows has a tile, so that rows that see nothing are written too.
+  auto weight_of = [&](const Work& w) { return w.rows > 0 ? max(w.tiles.count, 1) : 0; };
+
+  int seq, local, share = 0;
+  if (Args& a = fresh_args(); a.shares > 0) {
+    locate(
+        a.num_seqs, sm.loc,
+        [&](int s) {
+          return weight_of(work_of(make_seq(a, a.starts[s], a.starts[s + 1], a.lens[s], a.prefix != nullptr ? a.prefix[s] : 0)));
+        },
+        [&](int all) {
+          share = max((all + a.shares - 1) / a.shares, kMinShare);
+          return static_cast<int>(min(static_cast<int64_t>(g) * share, static_cast<int64_t>(all)));
+        },
+        seq, local);
+    if (seq < 0) return;
+  } else {
+    seq = g;
+    local = 0;
+  }
+  int left = share;
+
+  typename Smem::Tile& tile = sm.tile[wave];
+
+  for (;; ++seq, local = 0) {
+    Args& a = fresh_args();
+    if (seq >= a.num_seqs) return;
+    const char* kbase = static_cast<const char*>(a.k) + ELT * (static_cast<int64_t>(kv_head) * a.k_sh);
+    const char* vbase = static_cast<const char*>(a.v) + ELT * (static_cast<int64_t>(kv_head) * a.v_sh);
+    const Seq sq = make_seq(a, scalar_load(a.starts, seq), scalar_load(a.starts, seq + 1), scalar_load(a.lens, seq),
+                            a.prefix != nullptr ? scalar_load(a.prefix, seq) : 0);
+    const Work w = work_of(sq);
+    const int weight = weight_of(w);
+    if (weight == 0) {
+      if (share == 0) return;
+      continue;
+    }
+    const int u0 = local, u1 = share > 0 ? min(weight, local + left) : weight;
+    left -= u1 - u0;
+    // This lane's row (of the last one from there on).
+    const int row = min(l16, w.rows - 1);
+    const int tok = row / p.group;
+    const int q_head = kv_head * p.group + (row - tok * p.group);
+    const int pos = w.pos0 + tok;
+    u32x4 qf[CH];  // B operand: row l16, columns 32 c + 8 lg ...
+    {
+      const uint16_t* src = a.q + static_cast<int64_t>(sq.first + tok) * a.q_st + static_cast<int64_t>(q_head) * a.q_sh + 8 * lg;
+      const bool wide = (reinterpret_cast<uintptr_t>(a.q) % 16 == 0) && a.q_st % 8 == 0 && a.q_sh % 8 == 0;
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        if (wide) {
+          qf[c] = *reinterpret_cast<const u32x4*>(src + 32 * c);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            qf[c][e] = static_cast<uint32_t>(src[32 * c + 2 * e]) | static_cast<uint32_t>(src[32 * c + 2 * e + 1]) << 16;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) qf[c][e] ^= a.q_sign;
+      }
+    }
+    const float slope2 = a.slopes != nullptr ? a.slopes[q_head] * kLog2e : 0.0f;
+    auto used = [&](int j) { return j < sq.pre || (j >= w.lo && j < sq.len); };
+    auto page_at = [&](auto& c, int j) {
+      return min(max(c.tables[static_cast<int64_t>(seq) * c.bt_stride + div_block(c, j)], 0), c.num_blocks - 1);
+    };
+
+    f32x4 acc[NB];  // O^T: row l16, columns 16 b + 4 lg + i
+#pragma unroll
+    for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m_ref = -__builtin_huge_valf(), l_run = 0.0f;
+
+    struct Regs {
+      u32x4 k[TG * NI], v[TG * NI];
+    } buf[DEPTH];
+
+    int pages[TG];  // lane e: the cache block of this wave's e-th tile from c0 on (-1: no key of it is seen)
+    // The wave's i-th tile is u0 + wave + 4 i.
+    auto tile_at = [&](int i) { return w.tiles.index(u0 + wave + kTileWaves * i) * TT; };
+    auto load = [&](int i, int e, bool live, Regs& r) {
+      const int t0 = tile_at(i);
+      const bool inner = t0 + TT <= sq.pre || (t0 >= w.lo && t0 + TT <= sq.len);
+#pragma unroll
+      for (int h = 0; h < TG; ++h) {
+        const int r0 = t0 + 16 * h;
+        if constexpr (BS16) {
+          const int page = __builtin_amdgcn_readlane(pages[h], e);
+          const int nrec = live && page >= 0 ? 0x7fffffff : 0;
+          const int off = r0 - div_block(p, r0) * p.block_size;
+          const int64_t pg = page < 0 ? 0 : page;
+          const char* kt = kbase + ELT * (pg * p.k_sb + static_cast<int64_t>(off) * p.k_st);
+          const char* vt = vbase + ELT * (pg * p.v_sb + static_cast<int64_t>(off) * p.v_st);
+          const auto brk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kt), 0, nrec, kRsrcWord3);
+          const auto brv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vt), 0, nrec, kRsrcWord3);
+#pragma unroll
+          for (int x = 0; x < NI; ++x) {
+            const int o = 1024 * x + 16 * lane;
+            int ko = o / RB * p.k_st * ELT + o % RB;
+            if (!inner && !used(r0 + o / RB)) ko = -1;  // past num_records: zeros
+            r.k[NI * h + x] = __builtin_amdgcn_raw_buffer_load_b128(brk, ko, 0, 2);
+          }
+#pragma unroll
+          for (int x = 0; x < NI; ++x) {
+            const int o = 1024 * x + 16 * lane;
+            int vo = o / RB * p.v_st * ELT + o % RB;
+            if (!inner && !used(r0 + o / RB)) vo = -1;
+            r.v[NI * h + x] = __builtin_amdgcn_raw_buffer_load_b128(brv, vo, 0, 2);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < NI; ++x) {
+            const int o = 1024 * x + 16 * lane;
+            const int j = r0 + o / RB;
+            r.k[NI * h + x] = r.v[NI * h + x] = u32x4{0u, 0u, 0u, 0u};
+            if (live && used(j)) {
+              const int blk = div_block(p, j);
+              const int64_t page = page_at(p, j);
+              const int64_t off = j - blk * p.block_size;
+              r.k[NI * h + x] = *reinterpret_cast<const u32x4*>(kbase + ELT * (page * p.k_sb + off * p.k_st) + o % RB);
+              r.v[NI * h + x] = *reinterpret_cast<const u32x4*>(vbase + ELT * (page * p.v_sb + off * p.v_st) + o % RB);
+            }
+          }
+        }
+      }
+    };
+
+    auto consume = [&](int i, const Regs& r) {
+      const int t0 = tile_at(i);
+      // Every row sees all keys of the tile.
+      const bool full = t0 + TT <= sq.pre || (t0 + TT - 1 <= w.pos0 && t0 > sq.len - 1 - p.window);
+      // To LDS in the dtype; rows of one position hide the same keys from all.
+      bool bad = false;
+      const bool mixed = !full && sq.n > 1;
+#pragma unroll
+      for (int x = 0; x < TG * NI; ++x) {
+        const int o = 1024 * (x % NI) + 16 * lane;
+        const int rr = 16 * (x / NI) + o / RB, col = (o % RB) / ELT;
+        u32x4 v0, v1;
+        if constexpr (FP8) {
+          *reinterpret_cast<u32x4*>(tile.k + rr * P + col) = fp8x8_to<E>(u32x2{r.k[x][0], r.k[x][1]});
+          *reinterpret_cast<u32x4*>(tile.k + rr * P + col + 8) = fp8x8_to<E>(u32x2{r.k[x][2], r.k[x][3]});
+          v0 = fp8x8_to<E>(u32x2{r.v[x][0], r.v[x][1]});
+          v1 = fp8x8_to<E>(u32x2{r.v[x][2], r.v[x][3]});
+        } else {
+          *reinterpret_cast<u32x4*>(tile.k + rr * P + col) = r.k[x];
+          v0 = r.v[x];
+        }
+        if (mixed) {
+          uint32_t up, down;
+          v0 = take_out<E>(v0, up, down);
+          reinterpret_cast<uint8_t*>(tile.up[rr])[col / 8] = static_cast<uint8_t>(up);
+          reinterpret_cast<uint8_t*>(tile.down[rr])[col / 8] = static_cast<uint8_t>(down);
+          bad = bad || (up | down) != 0;
+          if constexpr (FP8) {
+            v1 = take_out<E>(v1, up, down);
+            reinterpret_cast<uint8_t*>(tile.up[rr])[col / 8 + 1] = static_cast<uint8_t>(up);
+            reinterpret_cast<uint8_t*>(tile.down[rr])[col / 8 + 1] = static_cast<uint8_t>(down);
+            bad = bad || (up | down) != 0;
+          }
+        }
+        *reinterpret_cast<u32x4*>(tile.v + rr * P + col) = v0;
+        if constexpr (FP8) *reinterpret_cast<u32x4*>(tile.v + rr * P + col + 8) = v1;
+      }
+      f32x4 s[TG];  // keys t0 + 16 h + 4 lg + i of row l16
+#pragma unroll
+      for (int h = 0; h < TG; ++h) {
+        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+          const u32x4 ka = *reinterpret_cast<const u32x4*>(tile.k + (16 * h + l16) * P + 8 * lg + 32 * c);
+          s[h] = E::mfma_16x16x32(ka, qf[c], s[h]);
+        }
+      }
+      float factor = p.scale2;
+      if (p.cap2 > 0.0f) {
+#pragma unroll
+        for (int h = 0; h < TG; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[h][e] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[h][e] * p.scale2) + 1.0f);
+        factor = 1.0f;
+      }
+      const int away0 = pos - t0 - 4 * lg;
+      float top = -__builtin_huge_valf();
+#pragma unroll
+      for (int h = 0; h < TG; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int at = 16 * h + e;
+          float x = s[h][e] * factor;
+          if (p.slopes != nullptr) x -= slope2 * static_cast<float>(abs(away0 - at));
+          if (!full) {
+            const bool sees = static_cast<uint32_t>(away0 - at) < static_cast<uint32_t>(p.window) || t0 + 4 * lg + at < sq.pre;
+            x = sees ? x : -__builtin_huge_valf();
+          }
+          s[h][e] = x;
+          top = fmaxf(top, x);
+        }
+      top = rows_max(top);
+      if (__any(top > m_ref + 8.0f)) {  // the reference follows only where a tile passes it by 2^8
+        const float m_new = fmaxf(m_ref, top);
+        const float alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -__builtin_huge_valf() ? 0.0f : m_new));
+        m_ref = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) acc[b] *= alpha;
+      }
+      const float ref = m_ref == -__builtin_huge_valf() ? 0.0f : m_ref;
+      // Weights as a sum of two parts of the dtype, exact to 2^-16: the products
+      // are a small part of a call that waits for memory.
+      u32x2 hi[TG], lo[TG];
+#pragma unroll
+      for (int h = 0; h < TG; ++h) {
+        float w4[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          w4[e] = __builtin_amdgcn_exp2f(s[h][e] - ref);
+          l_run += w4[e];
+        }
+        hi[h] = u32x2{pack2<E>(w4[0], w4[1]), pack2<E>(w4[2], w4[3])};
+        lo[h] = u32x2{pack2<E>(w4[0] - E::lo(hi[h][0]), w4[1] - E::hi(hi[h][0])),
+                      pack2<E>(w4[2] - E::lo(hi[h][1]), w4[3] - E::hi(hi[h][1]))};
+      }
+      const uint16_t* vt = tile.v + (4 * lg + l16 / 4) * P + 4 * (l16 % 4);
+#pragma unroll
+      for (int h = 0; h < TG; ++h)
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          using lds_v4i16 = __attribute__((address_space(3))) s16x4;
+          const u32x2 va = __builtin_bit_cast(
+              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + 16 * h * P + 16 * b)));
+          acc[b] = E::mfma_16x16x16(va, hi[h], acc[b]);
+          acc[b] = E::mfma_16x16x16(va, lo[h], acc[b]);
+        }
+      if (mixed && __any(bad)) {
+        // As in tile_kernel: a row takes the infinities whose key has a weight there.
+        uint32_t up[CH] = {}, down[CH] = {};
+#pragma unroll 1
+        for (int j = 0; j < TT; ++j) {
+          uint32_t word = 0;
+#pragma unroll
+          for (int h = 0; h < TG; ++h)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) word |= h == j / 16 && x == j % 4 / 2 ? hi[h][x] : 0u;
+          word = j % 2 != 0 ? word >> 16 : word & 0xffffu;
+          const uint32_t takes = __shfl(word, l16 + 16 * (j % 16 / 4), kWave) != 0 ? 0xffffffffu : 0u;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) {
+            up[c] |= tile.up[j][c] & takes;
+            down[c] |= tile.down[j][c] & takes;
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const int u = static_cast<int>(up[b / 2] >> (16 * (b % 2) + 4 * lg));
+          const int d = static_cast<int>(down[b / 2] >> (16 * (b % 2) + 4 * lg));
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            acc[b][e] += __int_as_float(((u << (31 - e)) >> 31) & 0x7f800000);
+            acc[b][e] -= __int_as_float(((d << (31 - e)) >> 31) & 0x7f800000);
+          }
+        }
+      }
+    };
+
+    const int count = min(u1, w.tiles.count) - u0;  // 0: no key is seen
+    const int mine = count > wave ? (count - wave + kTileWaves - 1) / kTileWaves : 0;
+    for (int c0 = 0; c0 < mine; c0 += kWave) {
+      const int m = min(mine - c0, kWave);
+      if constexpr (BS16) {
+        Args& c = fresh_args();
+#pragma unroll
+        for (int h = 0; h < TG; ++h) {
+          pages[h] = -1;
+          if (lane < m) {
+            const int r0 = tile_at(c0 + lane) + 16 * h;
+            if (r0 < sq.pre || (r0 + 16 > w.lo && r0 < sq.len)) pages[h] = page_at(c, r0);
+          }
+        }
+      }
+#pragma unroll
+      for (int d = 0; d < DEPTH; ++d) {
+        load(c0 + d, d, d < m, buf[d]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+      for (int i = 0; i < m; i += DEPTH) {
+#pragma unroll
+        for (int d = 0; d < DEPTH; ++d) {
+          if (i + d < m) consume(c0 + i + d, buf[d]);
+          // Past the end too, from no records, so that the waits stay for the oldest tile.
+          load(c0 + i + d + DEPTH, min(i + d + DEPTH, kWave - 1), i + d + DEPTH < m, buf[d]);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      }
+    }
+
+    // The waves' sums to one.
+    Args& b = fresh_args();
+    const float l_all = rows_sum(l_run);
+    lds_barrier();  // every wave has read its last tile
+    if (lg == 0) {
+      sm.m[wave][l16] = m_ref;
+      sm.l[wave][l16] = l_all;
+    }
+    if (l16 < w.rows) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) *reinterpret_cast<f32x4*>(&sm.o[wave][l16 * OP + 16 * n + 4 * lg]) = acc[n];
+    }
+    lds_barrier();
+    const bool whole = u0 == 0 && u1 == weight;
+    const int64_t slot = (static_cast<int64_t>(g + seq) * b.hkv + kv_head) * b.slot_rows;
+    if (!whole && u0 == 0 && tid == 0) {
+      int32_t* first = b.ws_first + 2 * (static_cast<int64_t>(seq) * b.hkv + kv_head);
+      first[0] = g;
+      first[1] = 1 + (weight - u1 + share - 1) / share;
+    } else if (whole && share > 0 && tid == 0) {
+      b.ws_first[2 * (static_cast<int64_t>(seq) * b.hkv + kv_head) + 1] = 0;
+    }
+    for (int idx = tid; idx < w.rows * (D / 4); idx += kTileThreads) {
+      const int r = idx / (D / 4), d = 4 * (idx % (D / 4));
+      float M = sm.m[0][r];
+#pragma unroll
+      for (int x = 1; x < kTileWaves; ++x) M = fmaxf(M, sm.m[x][r]);
+      const float ref = M == -__builtin_huge_valf() ? 0.0f : M;
+      float L = 0.0f;
+      f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int x = 0; x < kTileWaves; ++x) {
+        const float f = __builtin_amdgcn_exp2f(sm.m[x][r] - ref);
+        L += f * sm.l[x][r];
+        O += f * *reinterpret_cast<const f32x4*>(&sm.o[x][r * OP + d]);
+      }
+      if (whole) {
+        const int rt = r / b.group;
+        uint16_t* dst = b.out + static_cast<int64_t>(sq.first + rt) * b.o_st +
+                        static_cast<int64_t>(kv_head * b.group + r - rt * b.group) * b.o_sh + d;
+        store4<E>(b, dst, L == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : O * (b.v_scale / L));
+      } else {
+        *reinterpret_cast<f32x4*>(b.ws + (slot + r) * D + d) = O;
+        if (d == 0) {
+          b.ws_ml[2 * (slot + r)] = M;
+          b.ws_ml[2 * (slot + r) + 1] = L;
+        }
+      }
+    }
+    if (left <= 0) return;
+    lds_barrier();  // the sums have been read: the next piece's tiles may take their place
+  }
+}
+
+// Joins the pieces of row_kernel's cut sequences, in their order: a wave a row.
+template <typename E, int D>
+__global__ __launch_bounds__(kTileThreads) void row_join_kernel(const KParams p) {
+  constexpr int LD = D / 4;                        // lanes of a row
+  constexpr int SETS = kWave / LD > 0 ? kWave / LD : 1;  // pieces side by side
+  const int lane = threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) / kWave);
+  const int kv_head = static_cast<int>(blockIdx.x) % p.hkv;
+  const int seq = static_cast<int>(blockIdx.x) / p.hkv;
+  const int r = static_cast<int>(blockIdx.y) * kTileWaves + wave;
+  const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), 0, 0);
+  const int64_t rows = static_cast<int64_t>(sq.n) * p.group;
+  if (rows > kShortRows || r >= min(static_cast<int>(rows), p.slot_rows)) return;  // a tiled sequence, or no such row
+  const int64_t entry = 2 * (static_cast<int64_t>(seq) * p.hkv + kv_head);
+  const int g = p.ws_first[entry], count = p.ws_first[entry + 1];
+  if (count == 0) return;  // written whole
+  const int64_t slot = (static_cast<int64_t>(g + seq) * p.hkv + kv_head) * p.slot_rows + r;
+  const int64_t step = static_cast<int64_t>(p.hkv) * p.slot_rows;  // the next workgroup's slot
+  float M = -__builtin_huge_valf();
+  for (int i = lane; i < count; i += kWave) M = fmaxf(M, p.ws_ml[2 * (slot + i * step)]);
+  M = wave_max(M);
+  const float ref = M == -__builtin_huge_valf() ? 0.0f : M;
+  const int set = lane / LD, d = 4 * (lane % LD);
+  float L = 0.0f;
+  f32x4 O = {0.f, 0.f, 0.f, 0.f};
+  if (set < SETS) {
+#pragma unroll 4
+    for (int i = set; i < count; i += SETS) {
+      const float f = __builtin_amdgcn_exp2f(p.ws_ml[2 * (slot + i * step)] - ref);
+      L += f * p.ws_ml[2 * (slot + i * step) + 1];
+      O += f * *reinterpret_cast<const f32x4*>(p.ws + (slot + i * step) * D + d);
+    }
+  }
+#pragma unroll
+  for (int x = 1; x < SETS; ++x) {
+    const int from = lane % LD + x * LD;
+    const float l2 = __shfl(L, from, kWave);
+    const f32x4 o2 = {__shfl(O[0], from, kWave), __shfl(O[1], from, kWave), __shfl(O[2], from, kWave), __shfl(O[3], from, kWave)};
+    if (set == 0) {
+      L += l2;
+      O += o2;
+    }
+  }
+  if (set != 0) return;
+  const int rt = r / p.group;
+  uint16_t* dst = p.out + static_cast<int64_t>(sq.first + rt) * p.o_st +
+                  static_cast<int64_t>(kv_head * p.group + r - rt * p.group) * p.o_sh + d;
+  store4<E>(p, dst, L == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : O * (p.v_scale / L));
+}
+
+// How a call is cut, from what the host knows: the sizes and the bounds.
+struct Plan {
+  int64_t tile_groups = 0;  // workgroups of tile_kernel; 0: every sequence has few rows
+  int64_t row_groups = 0;   // and of row_kernel
+  int shares = 0, slot_rows = kShortRows;
+  int64_t slots = 0;        // row_kernel's
+  int64_t ws_bytes = 0;
+  int64_t ml_at = 0, first_at = 0;  // floats from the workspace's start
+};
+
+Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max_len, int window) {
+  Plan plan;
+  const int group = a->num_q_heads / a->num_kv_heads;
+  const int64_t hkv = a->num_kv_heads, rows = static_cast<int64_t>(a->num_tokens) * group;
+  const int64_t most_rows = static_cast<int64_t>(std::min(max_query_len, a->num_tokens)) * group;
+  if (most_rows > kShortRows) {
+    // At most this many row tiles: full ones, and one more a sequence, of at least 17 rows each.
+    const int64_t tiles = rows / kTileRows + std::min<int64_t>(a->num_seqs, rows / (kShortRows + 1));
+    plan.tile_groups = tiles * hkv;
+  }
+  plan.row_groups = a->num_seqs * hkv;
+  // Keys that a token may see, as far as the host knows.
+  const int64_t keys = a->prefix_lens != nullptr ? max_len : std::min<int64_t>(max_len, static_cast<int64_t>(window) + 16);
+  if (keys > kWholeKeys) {
+    const int64_t resident = d <= 64 ? 768 : d <= 128 ? 512 : 256;  // workgroups of row_kernel on 256 CUs
+    plan.shares = static_cast<int>(std::max<int64_t>(resident / hkv, 1));
+    plan.row_groups = plan.shares * hkv;
+    plan.slot_rows = static_cast<int>(std::min<int64_t>(most_rows, kShortRows));
+    plan.slots = (plan.shares + static_cast<int64_t>(a->num_seqs)) * hkv;
+    plan.ml_at = plan.slots * plan.slot_rows * d;
+    plan.first_at = plan.ml_at + plan.slots * plan.slot_rows * 2;
+    plan.ws_bytes = 4 * (plan.first_at + 2 * a->num_seqs * hkv);
+  }
+  return plan;
+}
+
+// The plan without a workspace: nothing is cut.
+Plan whole_plan(const dk_varlen_attn_params* a, const Plan& with) {
+  Plan plan;
+  plan.tile_groups = with.tile_groups;
+  plan.row_groups = static_cast<int64_t>(a->num_seqs) * a->num_kv_heads;
+  return plan;
+}
+
 template <typename E, int D, bool FP8>
-hipError_t launch_tiles(const KParams& kp, hipStream_t s) {
-  // At most this many row tiles: full ones, and one more a sequence (at least 17 rows each).
-  const int64_t rows = static_cast<int64_t>(kp.num_tokens) * kp.group;
-  const int64_t more = std::min<int64_t>(kp.num_seqs, rows / (kp.rows_short + 1));
-  const int64_t bound = rows / kTileRows + more;
-  const dim3 grid(static_cast<unsigned>(bound * kp.hkv)), block(kTileThreads);
-  const int64_t reach = int64_t{16} * 2 * std::max(kp.k_st, kp.v_st);
-  if (kp.block_size % 16 == 0 && reach < (int64_t{1} << 31))
-    hipLaunchKernelGGL((tile_kernel<E, D, FP8, true>), grid, block, 0, s, kp);
-  else hipLaunchKernelGGL((tile_kernel<E, D, FP8, false>), grid, block, 0, s, kp);
+hipError_t launch_all(const KParams& kp, const Plan& plan, hipStream_t s) {
+  const dim3 block(kTileThreads);
+  // Rows of a 16-key group within the 2^31 bytes of a buffer resource.
+  const bool bs16 = kp.block_size % 16 == 0 && int64_t{16} * 2 * std::max(kp.k_st, kp.v_st) < (int64_t{1} << 31);
+  if (plan.tile_groups > 0) {
+    const dim3 grid(static_cast<unsigned>(plan.tile_groups));
+    if (bs16) hipLaunchKernelGGL((tile_kernel<E, D, FP8, true>), grid, block, 0, s, kp);
+    else hipLaunchKernelGGL((tile_kernel<E, D, FP8, false>), grid, block, 0, s, kp);
+  }
+  {
+    const dim3 grid(static_cast<unsigned>(plan.row_groups));
+    if (bs16) hipLaunchKernelGGL((row_kernel<E, D, FP8, true>), grid, block, 0, s, kp);
+    else hipLaunchKernelGGL((row_kernel<E, D, FP8, false>), grid, block, 0, s, kp);
+    if (kp.shares > 0) {
+      const dim3 join(static_cast<unsigned>(kp.num_seqs * kp.hkv), static_cast<unsigned>((kp.slot_rows + 3) / 4));
+      hipLaunchKernelGGL((row_join_kernel<E, D>), join, block, 0, s, kp);
+    }
+  }
   return hipGetLastError();
 }
 
 template <typename E>
-hipError_t launch(const KParams& kp, int d, int max_query_len, bool fp8, hipStream_t s) {
-  if (static_cast<int64_t>(max_query_len) * kp.group > kp.rows_short) {
-    hipError_t e = hipSuccess;
-    if (fp8) {
-      switch (d) {
-        case 64: e = launch_tiles<E, 64, true>(kp, s); break;
-        case 128: e = launch_tiles<E, 128, true>(kp, s); break;
-        case 192: e = launch_tiles<E, 192, true>(kp, s); break;
-        default: e = launch_tiles<E, 256, true>(kp, s); break;
-      }
-    } else {
-      switch (d) {
-        case 64: e = launch_tiles<E, 64, false>(kp, s); break;
-        case 96: e = launch_tiles<E, 96, false>(kp, s); break;
-        case 128: e = launch_tiles<E, 128, false>(kp, s); break;
-        case 192: e = launch_tiles<E, 192, false>(kp, s); break;
-        default: e = launch_tiles<E, 256, false>(kp, s); break;
-      }
+hipError_t launch(const KParams& kp, const Plan& plan, int d, bool fp8, hipStream_t s) {
+  if (fp8) {
+    switch (d) {
+      case 64: return launch_all<E, 64, true>(kp, plan, s);
+      case 128: return launch_all<E, 128, true>(kp, plan, s);
+      case 192: return launch_all<E, 192, true>(kp, plan, s);
+      default: return launch_all<E, 256, true>(kp, plan, s);
     }
-    if (e != hipSuccess) return e;
   }
-  const dim3 grid(static_cast<unsigned>(kp.num_tokens * kp.hq)), block(kWave);
-  if (fp8) hipLaunchKernelGGL((simple_kernel<E, true>), grid, block, 0, s, kp, d);
-  else hipLaunchKernelGGL((simple_kernel<E, false>), grid, block, 0, s, kp, d);
-  return hipGetLastError();
+  switch (d) {
+    case 64: return launch_all<E, 64, false>(kp, plan, s);
+    case 96: return launch_all<E, 96, false>(kp, plan, s);
+    case 128: return launch_all<E, 128, false>(kp, plan, s);
+    case 192: return launch_all<E, 192, false>(kp, plan, s);
+    default: return launch_all<E, 256, false>(kp, plan, s);
+  }
+}
+
+// No length goes past the caller's bound and what the block tables hold.
+int length_bound(const dk_varlen_attn_params* a, int max_seq_len) {
+  const int64_t held = static_cast<int64_t>(a->max_blocks) * a->block_size;
+  return a->num_blocks == 0 ? 0 : static_cast<int>(std::min<int64_t>(held, max_seq_len));
+}
+
+int window_bound(const dk_varlen_attn_params* a, int max_len) {
+  return a->window == 0 || a->window > max_len ? std::max(max_len, 1) : a->window;
 }
 
 int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim, int max_query_len, int max_seq_len,
@@ -776,8 +1254,7 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
   if (a->num_tokens == 0 || a->num_seqs == 0) return hipSuccess;
   if (a->out == nullptr || a->q == nullptr || a->seq_lens == nullptr || a->query_start_loc == nullptr)
     return fail("%s: out, q, seq_lens and query_start_loc must not be NULL", op);
-  const int64_t held = static_cast<int64_t>(a->max_blocks) * a->block_size;
-  const int max_len = a->num_blocks == 0 ? 0 : static_cast<int>(held < max_seq_len ? held : max_seq_len);
+  const int max_len = length_bound(a, max_seq_len);
   if (max_len > 0 && (a->k_cache == nullptr || a->v_cache == nullptr || a->block_tables == nullptr))
     return fail("%s: k_cache, v_cache and block_tables must not be NULL", op);
   for (const int64_t stride :
@@ -819,28 +1296,32 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
   kp.block_size = a->block_size;
   kp.num_blocks = a->num_blocks;
   kp.max_len = max_len;
-  kp.window = a->window == 0 || a->window > max_len ? (max_len > 0 ? max_len : 1) : a->window;
-  kp.scale = a->scale;
-  kp.softcap = a->softcap;
-  kp.k_scale = k_scale;
+  kp.window = window_bound(a, max_len);
   kp.v_scale = v_scale;
-  (void)workspace, (void)workspace_bytes;
   kp.hkv = a->num_kv_heads;
-  kp.rows_short = 16;
+  Plan plan = make_plan(a, head_dim, max_query_len, max_len, kp.window);
+  if (plan.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < plan.ws_bytes)) plan = whole_plan(a, plan);
+  if (plan.ws_bytes > 0 && !aligned_to(workspace, 16)) return fail("%s: workspace must be 16-byte aligned", op);
+  if (plan.tile_groups > 0x7fffffff || plan.row_groups > 0x7fffffff || static_cast<int64_t>(a->num_seqs) * a->num_kv_heads > 0x7fffffff)
+    return fail("%s: too many sequences x heads", op);
+  kp.shares = plan.shares;
+  kp.slot_rows = plan.slot_rows;
+  kp.ws = static_cast<float*>(workspace);
+  kp.ws_ml = kp.ws + plan.ml_at;
+  kp.ws_first = reinterpret_cast<int32_t*>(kp.ws + plan.first_at);
   // floor(j / b) = (j * ceil(2^k / b)) >> k for j < 2^31 with k = 31 + ceil(log2 b):
   // the factor is off by less than 1, the product by less than 2^31 <= 2^k / b.
   int k = 31;
   while ((int64_t{1} << (k - 31)) < a->block_size) ++k;
   kp.bs_shift = k;
   kp.bs_mul = static_cast<uint32_t>(((uint64_t{1} << k) + a->block_size - 1) / a->block_size);
-  const float c = kp.scale * kp.k_scale;
+  const float c = a->scale * k_scale;
   kp.q_sign = c < 0.0f ? 0x80008000u : 0u;
-  kp.scale2 = std::fabs(c) * kLog2e;
-  kp.cap2 = kp.softcap * kLog2e;
-  kp.cap_in = kp.softcap > 0.0f ? 2.0f * kLog2e * std::fabs(c) / kp.softcap : 0.0f;
+  kp.cap2 = a->softcap * kLog2e;
+  kp.scale2 = std::fabs(c) * kLog2e * (a->softcap > 0.0f ? 2.0f / a->softcap : 1.0f);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  return static_cast<int>(dtype == DK_BFLOAT16 ? launch<Bf16>(kp, head_dim, max_query_len, fp8, s)
-                                               : launch<F16>(kp, head_dim, max_query_len, fp8, s));
+  return static_cast<int>(dtype == DK_BFLOAT16 ? launch<Bf16>(kp, plan, head_dim, fp8, s)
+                                               : launch<F16>(kp, plan, head_dim, fp8, s));
 }
 
 }  // namespace varlen
@@ -848,8 +1329,12 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
 
 extern "C" int64_t dk_paged_attention_varlen_workspace_bytes(const dk_varlen_attn_params* a, int head_dim,
                                                              int max_query_len, int max_seq_len) {
-  (void)a, (void)head_dim, (void)max_query_len, (void)max_seq_len;
-  return 0;
+  using namespace dk::varlen;
+  if (a == nullptr || a->num_kv_heads <= 0 || a->num_q_heads < a->num_kv_heads || a->num_tokens <= 0 || a->num_seqs <= 0 ||
+      max_query_len < 0 || max_seq_len < 0 || a->num_blocks < 0 || a->max_blocks < 0 || a->block_size <= 0 || head_dim <= 0)
+    return 0;  // nothing to do, or refused by the call
+  const int max_len = length_bound(a, max_seq_len);
+  return make_plan(a, head_dim, max_query_len, max_len, window_bound(a, max_len)).ws_bytes;
 }
 
 extern "C" int dk_paged_attention_varlen(const dk_varlen_attn_params* a, int dtype, int head_dim, int max_query_len,

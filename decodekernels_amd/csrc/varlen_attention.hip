@@ -41,12 +41,15 @@ struct KParams {
   int hkv;
   int split_items;         // tile_kernel: workgroups that the tiles of a call may be split over; 0: never split
   int shares;              // row_kernel: workgroups a KV head, of equal shares of all key tiles; 0: one a sequence
-  int slot_rows;           // row_kernel: rows of a slot
-  float* ws;               // partial results: sums, row by row of a slot
-  float* ws_ml;            // their reference maximum (log2 units) and exp-sum
+  int short_rows;          // rows of a KV head up to which a sequence runs in row_kernel: 16 or 32
+  int slot_rows;           // row_kernel: rows of a slot, as many as max_query_len allows
+  // Partial results, row by row of an item or slot: sums, and their reference
+  // maximum (log2 units) and exp-sum.
+  float *tile_ws, *tile_ml, *ws, *ws_ml;
   int32_t* ws_first;       // row_kernel: a sequence's first workgroup, and how many
   uint32_t bs_mul;         // j / block_size = (j * bs_mul) >> bs_shift, for j < 2^31
   int bs_shift;
+  int biased;              // slopes are given
   float v_scale;           // of an fp8 cache (1 otherwise)
   // In log2 units: the cap (0: none) and the positive factor of q.k, whose sign
   // goes to q: the score's, or with a cap that of the exponent of e^(2 y) in
@@ -78,15 +81,14 @@ __device__ __forceinline__ f32x16 mfma_32x32x16<F16>(u32x4 a, u32x4 b, f32x16 c)
   return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Rows of a KV head, (token, query head of its group) pairs, up to which a
-// sequence runs in row_kernel, which has one 16-column MFMA operand for them.
-constexpr int kShortRows = 16;
 constexpr int kTileWaves = 4;
 constexpr int kTileThreads = kTileWaves * kWave;
 constexpr int kTileRows = 32 * kTileWaves;  // (token, query head of the group) rows of a workgroup
 constexpr int kRsrcWord3 = 0x00020000;      // word 3 of a gfx9-family buffer resource for raw loads
 constexpr int kSeqsPerThread = 4;
 constexpr int kWholeKeys = 512;             // keys up to which a sequence of few rows is never cut
+constexpr int kMinPart = 8;                 // key tiles of a part of a row tile at least
+constexpr int kWideRows = 192;              // head_dim up to which row_kernel takes 32 rows: 256 has no registers for them
 constexpr int kMinShare = 16;               // key tiles a workgroup of row_kernel takes at least
 
 // Infinities and NaN of the dtype: the exponent bits of an element, and the
@@ -196,7 +198,7 @@ __device__ __forceinline__ void store4(const Params& p, uint16_t* dst, f32x4 y) 
 __device__ __forceinline__ int row_tiles(const KParams& p, int start, int end) {
   const int first = min(max(start, 0), p.num_tokens);
   const int64_t rows = static_cast<int64_t>(max(min(end, p.num_tokens) - first, 0)) * p.group;
-  return rows > kShortRows ? static_cast<int>((rows + kTileRows - 1) / kTileRows) : 0;
+  return rows > p.short_rows ? static_cast<int>((rows + kTileRows - 1) / kTileRows) : 0;
 }
 
 // Sequences s0 .. s0 + 1023, 4 a thread: weight(s) units each. Sets w and the
@@ -281,6 +283,33 @@ __device__ __forceinline__ KeyTiles key_tiles(int pre, int lo, int hi) {
   return k;
 }
 
+// A row tile of a sequence: its rows, the positions of the first and the last,
+// the keys that some row sees besides the prefix, and the key tiles that hold them.
+template <int TK>
+struct RowTile {
+  int row0, rows, pos0, pos1, lo, hi;
+  KeyTiles tiles;
+  __device__ __forceinline__ RowTile(const KParams& p, const Seq& sq, int local) {
+    row0 = local * kTileRows;
+    rows = min(sq.n * p.group - row0, kTileRows);
+    pos0 = sq.len - sq.n + row0 / p.group;
+    pos1 = sq.len - sq.n + (row0 + rows - 1) / p.group;
+    lo = max(pos0 - p.window + 1, 0);
+    hi = max(pos1 + 1, 0);
+    tiles = key_tiles<TK>(sq.pre, lo, hi);
+  }
+  // Key tiles of one of `parts` parts.
+  __device__ __forceinline__ int per_part(int parts) const {
+    return parts > 1 ? max((tiles.count + parts - 1) / parts, kMinPart) : tiles.count;
+  }
+};
+
+// Workgroups over which the key tiles of a row tile are spread, so that all
+// make up to split_items.
+__device__ __forceinline__ int parts_of(const KParams& p, int total) {
+  return p.split_items > 0 && total > 0 ? max(p.split_items / (total * p.hkv), 1) : 1;
+}
+
 template <int D>
 struct TileSmem {
   static constexpr int TK = tile_keys<D>();
@@ -334,7 +363,7 @@ void tile_kernel(const KParams p) {
   locate(
       p.num_seqs, loc, [&](int s) { return row_tiles(p, p.starts[s], p.starts[s + 1]); },
       [&](int total) {
-        if (p.split_items > 0 && total > 0) parts = max(p.split_items / (total * p.hkv), 1);
+        parts = parts_of(p, total);
         return item / p.hkv / parts;
       },
       seq, local);
@@ -342,21 +371,17 @@ void tile_kernel(const KParams p) {
   if (seq < 0) return;
   const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), scalar_load(p.lens, seq),
                           p.prefix != nullptr ? scalar_load(p.prefix, seq) : 0);
-  const int row0 = local * kTileRows;
-  const int rows = min(sq.n * p.group - row0, kTileRows);
-  // Positions of the workgroup's first and last row, and of this wave's.
-  const int pos0 = sq.len - sq.n + row0 / p.group;
-  const int pos1 = sq.len - sq.n + (row0 + rows - 1) / p.group;
+  const RowTile<TK> rt(p, sq, local);
+  const int row0 = rt.row0, rows = rt.rows, pos0 = rt.pos0, pos1 = rt.pos1, lo = rt.lo, hi = rt.hi;
+  const KeyTiles tiles = rt.tiles;
+  const int per = rt.per_part(parts);
+  const int n0 = min(part * per, tiles.count), n1 = min(n0 + per, tiles.count);
+  if (parts > 1 && part > 0 && n0 == n1) return;  // fewer parts than asked for
+  // Positions of this wave's first and last row.
   const int wave_row0 = min(32 * wave, rows - 1), wave_row1 = min(32 * wave + 31, rows - 1);
   const bool wave_live = 32 * wave < rows;
   const int wpos0 = sq.len - sq.n + (row0 + wave_row0) / p.group;
   const int wpos1 = sq.len - sq.n + (row0 + wave_row1) / p.group;
-  const int lo = max(pos0 - p.window + 1, 0), hi = max(pos1 + 1, 0);
-  const KeyTiles tiles = key_tiles<TK>(sq.pre, lo, hi);
-  // This part's tiles: at least 4, but for the last one's.
-  const int per = parts > 1 ? max((tiles.count + parts - 1) / parts, 4) : tiles.count;
-  const int n0 = min(part * per, tiles.count), n1 = min(n0 + per, tiles.count);
-
   // This lane's row; rows past the last one repeat it and are not stored.
   const int row = row0 + min(32 * wave + l32, rows - 1);
   const int tok = row / p.group;
@@ -641,10 +666,10 @@ void tile_kernel(const KParams p) {
   if (parts > 1) {
     // Partial results: sums against m_ref, joined by tile_join_kernel.
     const int64_t slot = (static_cast<int64_t>(item) * kTileRows) + 32 * wave + l32;
-    float* dst = p.ws + slot * D;
+    float* dst = p.tile_ws + slot * D;
     if (half == 0) {
-      p.ws_ml[2 * slot] = m_ref;
-      p.ws_ml[2 * slot + 1] = l_run;
+      p.tile_ml[2 * slot] = m_ref;
+      p.tile_ml[2 * slot + 1] = l_run;
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
@@ -666,9 +691,58 @@ void tile_kernel(const KParams p) {
 }
 
 
+// Joins the parts of row tiles over which tile_kernel was spread, in their
+// order. Workgroup (x, y) takes 16 rows of tile x / hkv, KV head x % hkv.
+template <typename E, int D>
+__global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams p) {
+  constexpr int LD = D / 4;                  // lanes of a row
+  constexpr int RS = kTileThreads / LD;      // rows side by side
+  __shared__ LocateSmem loc;
+  int seq, local, parts = 1;
+  const int kv_head = static_cast<int>(blockIdx.x) % p.hkv;
+  const int item0 = static_cast<int>(blockIdx.x) / p.hkv;
+  locate(
+      p.num_seqs, loc, [&](int s) { return row_tiles(p, p.starts[s], p.starts[s + 1]); },
+      [&](int total) {
+        parts = parts_of(p, total);
+        return item0;
+      },
+      seq, local);
+  if (seq < 0 || parts == 1) return;
+  const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), scalar_load(p.lens, seq),
+                          p.prefix != nullptr ? scalar_load(p.prefix, seq) : 0);
+  const RowTile<tile_keys<D>()> rt(p, sq, local);
+  const int per = rt.per_part(parts);
+  const int used = max((rt.tiles.count + per - 1) / per, 1);
+  const int d = 4 * (static_cast<int>(threadIdx.x) % LD);
+  for (int r = 16 * static_cast<int>(blockIdx.y) + static_cast<int>(threadIdx.x) / LD;
+       r < min(16 * static_cast<int>(blockIdx.y) + 16, rt.rows); r += RS) {
+    if (static_cast<int>(threadIdx.x) >= RS * LD) break;
+    // Part i's item is (item0 parts + i) hkv + the KV head, counted from the last (tile_kernel).
+    const int64_t slot = (static_cast<int64_t>(item0) * parts * p.hkv + (p.hkv - 1 - kv_head)) * kTileRows + r;
+    const int64_t step = static_cast<int64_t>(p.hkv) * kTileRows;
+    float M = -__builtin_huge_valf();
+#pragma unroll 4
+    for (int i = 0; i < used; ++i) M = fmaxf(M, p.tile_ml[2 * (slot + i * step)]);
+    const float ref = M == -__builtin_huge_valf() ? 0.0f : M;
+    float L = 0.0f;
+    f32x4 O = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int i = 0; i < used; ++i) {
+      const float f = __builtin_amdgcn_exp2f(p.tile_ml[2 * (slot + i * step)] - ref);
+      L += f * p.tile_ml[2 * (slot + i * step) + 1];
+      O += f * *reinterpret_cast<const f32x4*>(p.tile_ws + (slot + i * step) * D + d);
+    }
+    const int row = rt.row0 + r, tok = row / p.group;
+    uint16_t* dst = p.out + static_cast<int64_t>(sq.first + tok) * p.o_st +
+                    static_cast<int64_t>(kv_head * p.group + row - tok * p.group) * p.o_sh + d;
+    store4<E>(p, dst, L == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : O * (p.v_scale / L));
+  }
+}
+
 // LDS of row_kernel: each wave's current key tile, then, at the end of a piece,
 // the waves' sums in the same place.
-template <int D, bool FP8>
+template <int D, int R, bool FP8>
 struct RowSmem {
   static constexpr int TT = FP8 ? 32 : 16;  // keys of a tile: as many bytes in flight with either cache
   static constexpr int P = D + 16;          // row pitch, elements: 4 rows on distinct banks for the transpose reads
@@ -680,44 +754,45 @@ struct RowSmem {
   };
   union {
     Tile tile[kTileWaves];
-    float o[kTileWaves][kShortRows * OP];
+    float o[kTileWaves][16 * R * OP];
   };
-  float m[kTileWaves][kShortRows], l[kTileWaves][kShortRows];
+  float m[kTileWaves][16 * R], l[kTileWaves][16 * R];
   LocateSmem loc;
 };
 
-template <int D, bool FP8>
+template <int D, int R>
 constexpr int row_occupancy() {  // waves per SIMD
-  return D <= 64 ? 3 : D <= 128 ? 2 : 1;
+  return D <= 64 ? (R == 1 ? 3 : 2) : D <= 128 ? 2 : 1;
 }
 
-// Decode and speculation: up to 16 rows a KV head. Bound by the reading of the
+// Decode and speculation: up to 16 R rows a KV head (R = 1 or 2). Bound by the reading of the
 // cache, so all rows take each key tile once, a wave streams whole rows of its
 // own tiles (two in flight in registers) and the work is cut over the cache's
 // length: with `shares`, workgroup g of a KV head takes the g-th of equal
 // shares of all sequences' key tiles, whatever their lengths. A piece that is
 // not a whole sequence leaves its sums in slot g + s (sequence s; no two pieces
 // share one) for row_join_kernel. Scores are S^T = K Q^T and the output O^T =
-// V^T P^T on 16x16 MFMAs: lane l holds row l % 16 of both.
-template <typename E, int D, bool FP8, bool BS16>
+// V^T P^T on 16x16 MFMAs: lane l holds rows l % 16 (and + 16) of both.
+template <typename E, int D, int R, bool FP8, bool BS16>
 __global__ __launch_bounds__(kTileThreads)
-__attribute__((amdgpu_waves_per_eu(row_occupancy<D, FP8>(), row_occupancy<D, FP8>())))
+__attribute__((amdgpu_waves_per_eu(row_occupancy<D, R>(), row_occupancy<D, R>())))
 void row_kernel(const KParams p) {
-  using Smem = RowSmem<D, FP8>;
+  using Smem = RowSmem<D, R, FP8>;
   constexpr int TT = Smem::TT, P = Smem::P, OP = Smem::OP;
   constexpr int TG = TT / 16;           // 16-key groups of a tile: each lies in one cache block (BS16)
   constexpr int CH = D / 32, NB = D / 16;
   constexpr int ELT = FP8 ? 1 : 2;
   constexpr int RB = D * ELT;           // bytes of a K (or V) row
   constexpr int NI = 16 * RB / 1024;    // 16-byte loads of a lane for a group of K (or V)
-  constexpr int DEPTH = 2;
+  constexpr int DEPTH = 2;              // tiles in flight
   __shared__ Smem sm;
   const int tid = threadIdx.x;
   const int lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int l16 = lane % 16, lg = lane / 16;
-  const int kv_head = static_cast<int>(blockIdx.x) % p.hkv;
-  const int g = static_cast<int>(blockIdx.x) / p.hkv;
+  // Workgroup g of a KV head (formed where they are used, as the arguments).
+  auto head_of = [](Args& x) { return static_cast<int>(blockIdx.x) % x.hkv; };
+  auto group_of = [](Args& x) { return static_cast<int>(blockIdx.x) / x.hkv; };
 
   struct Work {
     Seq sq;
@@ -729,7 +804,7 @@ void row_kernel(const KParams p) {
     w.sq = sq;
     const int64_t rows = static_cast<int64_t>(sq.n) * p.group;
     // (slot_rows: no more than the caller's bound on the new tokens allows.)
-    w.rows = rows <= kShortRows ? min(static_cast<int>(rows), fresh_args().slot_rows) : 0;
+    w.rows = rows <= 16 * R ? min(static_cast<int>(rows), fresh_args().slot_rows) : 0;
     w.pos0 = sq.len - sq.n;
     w.lo = max(w.pos0 - p.window + 1, 0);
     w.tiles = key_tiles<TT>(sq.pre, w.lo, sq.len);
@@ -747,12 +822,12 @@ void row_kernel(const KParams p) {
         },
         [&](int all) {
           share = max((all + a.shares - 1) / a.shares, kMinShare);
-          return static_cast<int>(min(static_cast<int64_t>(g) * share, static_cast<int64_t>(all)));
+          return static_cast<int>(min(static_cast<int64_t>(group_of(a)) * share, static_cast<int64_t>(all)));
         },
         seq, local);
     if (seq < 0) return;
   } else {
-    seq = g;
+    seq = group_of(fresh_args());
     local = 0;
   }
   int left = share;
@@ -762,6 +837,7 @@ void row_kernel(const KParams p) {
   for (;; ++seq, local = 0) {
     Args& a = fresh_args();
     if (seq >= a.num_seqs) return;
+    const int kv_head = head_of(a);
     const char* kbase = static_cast<const char*>(a.k) + ELT * (static_cast<int64_t>(kv_head) * a.k_sh);
     const char* vbase = static_cast<const char*>(a.v) + ELT * (static_cast<int64_t>(kv_head) * a.v_sh);
     const Seq sq = make_seq(a, scalar_load(a.starts, seq), scalar_load(a.starts, seq + 1), scalar_load(a.lens, seq),
@@ -774,38 +850,53 @@ void row_kernel(const KParams p) {
     }
     const int u0 = local, u1 = share > 0 ? min(weight, local + left) : weight;
     left -= u1 - u0;
-    // This lane's row (of the last one from there on).
-    const int row = min(l16, w.rows - 1);
-    const int tok = row / p.group;
-    const int q_head = kv_head * p.group + (row - tok * p.group);
-    const int pos = w.pos0 + tok;
-    u32x4 qf[CH];  // B operand: row l16, columns 32 c + 8 lg ...
-    {
-      const uint16_t* src = a.q + static_cast<int64_t>(sq.first + tok) * a.q_st + static_cast<int64_t>(q_head) * a.q_sh + 8 * lg;
-      const bool wide = (reinterpret_cast<uintptr_t>(a.q) % 16 == 0) && a.q_st % 8 == 0 && a.q_sh % 8 == 0;
+    const bool whole = u0 == 0 && u1 == weight;
+    if (share > 0 && u0 == 0 && tid == 0) {  // for row_join_kernel: the first of its pieces' workgroups, and how many
+      int32_t* first = a.ws_first + 2 * (static_cast<int64_t>(seq) * a.hkv + kv_head);
+      first[0] = group_of(a);
+      first[1] = whole ? 0 : 1 + (weight - u1 + share - 1) / share;
+    }
+    // This lane's rows (the last one from there on).
+    int q_head[R], pos[R];
+    u32x4 qf[R][CH];  // B operand: row 16 r + l16, columns 32 c + 8 lg ...
+    float slope2[R];
+    const bool wide = (reinterpret_cast<uintptr_t>(a.q) % 16 == 0) && a.q_st % 8 == 0 && a.q_sh % 8 == 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const int row = min(16 * r + l16, w.rows - 1);
+      const int tok = row / a.group;
+      q_head[r] = kv_head * a.group + (row - tok * a.group);
+      pos[r] = w.pos0 + tok;
+      const uint16_t* src =
+          a.q + static_cast<int64_t>(sq.first + tok) * a.q_st + static_cast<int64_t>(q_head[r]) * a.q_sh + 8 * lg;
 #pragma unroll
       for (int c = 0; c < CH; ++c) {
         if (wide) {
-          qf[c] = *reinterpret_cast<const u32x4*>(src + 32 * c);
+          qf[r][c] = *reinterpret_cast<const u32x4*>(src + 32 * c);
         } else {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            qf[c][e] = static_cast<uint32_t>(src[32 * c + 2 * e]) | static_cast<uint32_t>(src[32 * c + 2 * e + 1]) << 16;
+            qf[r][c][e] = static_cast<uint32_t>(src[32 * c + 2 * e]) | static_cast<uint32_t>(src[32 * c + 2 * e + 1]) << 16;
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) qf[c][e] ^= a.q_sign;
+        for (int e = 0; e < 4; ++e) qf[r][c][e] ^= a.q_sign;
       }
+      slope2[r] = a.slopes != nullptr ? a.slopes[q_head[r]] * kLog2e : 0.0f;
     }
-    const float slope2 = a.slopes != nullptr ? a.slopes[q_head] * kLog2e : 0.0f;
     auto used = [&](int j) { return j < sq.pre || (j >= w.lo && j < sq.len); };
     auto page_at = [&](auto& c, int j) {
       return min(max(c.tables[static_cast<int64_t>(seq) * c.bt_stride + div_block(c, j)], 0), c.num_blocks - 1);
     };
 
-    f32x4 acc[NB];  // O^T: row l16, columns 16 b + 4 lg + i
+    f32x4 acc[R][NB];  // O^T: row 16 r + l16, columns 16 b + 4 lg + i
+    float m_ref[R], l_run[R];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) acc[b] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m_ref = -__builtin_huge_valf(), l_run = 0.0f;
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+      for (int b = 0; b < NB; ++b) acc[r][b] = f32x4{0.f, 0.f, 0.f, 0.f};
+      m_ref[r] = -__builtin_huge_valf();
+      l_run[r] = 0.0f;
+    }
 
     struct Regs {
       u32x4 k[TG * NI], v[TG * NI];
@@ -861,13 +952,14 @@ void row_kernel(const KParams p) {
       }
     };
 
-    auto consume = [&](int i, const Regs& r) {
-      const int t0 = tile_at(i);
-      // Every row sees all keys of the tile.
-      const bool full = t0 + TT <= sq.pre || (t0 + TT - 1 <= w.pos0 && t0 > sq.len - 1 - p.window);
-      // To LDS in the dtype; rows of one position hide the same keys from all.
+    // Every row sees all keys of the tile from t0 on.
+    auto all_see = [&](int t0) { return t0 + TT <= sq.pre || (t0 + TT - 1 <= w.pos0 && t0 > sq.len - 1 - p.window); };
+    // Tile i to LDS in the dtype. Where some rows see a key and others do not
+    // (not where all are of one position), infinities and NaN of V are taken
+    // out; whether this lane had any.
+    auto stage = [&](int i, const Regs& r) {
       bool bad = false;
-      const bool mixed = !full && sq.n > 1;
+      const bool mixed = sq.n > 1 && !all_see(tile_at(i));
 #pragma unroll
       for (int x = 0; x < TG * NI; ++x) {
         const int o = 1024 * (x % NI) + 16 * lane;
@@ -898,65 +990,76 @@ void row_kernel(const KParams p) {
         *reinterpret_cast<u32x4*>(tile.v + rr * P + col) = v0;
         if constexpr (FP8) *reinterpret_cast<u32x4*>(tile.v + rr * P + col + 8) = v1;
       }
-      f32x4 s[TG];  // keys t0 + 16 h + 4 lg + i of row l16
+      return bad;
+    };
+
+    auto consume = [&](int i, bool bad) {
+      const int t0 = tile_at(i);
+      const bool full = all_see(t0);
+      f32x4 s[R][TG];  // keys t0 + 16 h + 4 lg + i of row 16 r + l16
 #pragma unroll
       for (int h = 0; h < TG; ++h) {
-        s[h] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < R; ++x) s[x][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
           const u32x4 ka = *reinterpret_cast<const u32x4*>(tile.k + (16 * h + l16) * P + 8 * lg + 32 * c);
-          s[h] = E::mfma_16x16x32(ka, qf[c], s[h]);
+#pragma unroll
+          for (int x = 0; x < R; ++x) s[x][h] = E::mfma_16x16x32(ka, qf[x][c], s[x][h]);
         }
       }
-      float factor = p.scale2;
-      if (p.cap2 > 0.0f) {
+      // Weights as a sum of two parts of the dtype, exact to 2^-16: the products
+      // are a small part of a call that waits for memory.
+      u32x2 hi[R][TG], lo[R][TG];
+#pragma unroll
+      for (int x = 0; x < R; ++x) {
+        float factor = p.scale2;
+        if (p.cap2 > 0.0f) {
+#pragma unroll
+          for (int h = 0; h < TG; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[x][h][e] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[x][h][e] * p.scale2) + 1.0f);
+          factor = 1.0f;
+        }
+        const int away0 = pos[x] - t0 - 4 * lg;
+        float top = -__builtin_huge_valf();
 #pragma unroll
         for (int h = 0; h < TG; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[h][e] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[h][e] * p.scale2) + 1.0f);
-        factor = 1.0f;
-      }
-      const int away0 = pos - t0 - 4 * lg;
-      float top = -__builtin_huge_valf();
-#pragma unroll
-      for (int h = 0; h < TG; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int at = 16 * h + e;
-          float x = s[h][e] * factor;
-          if (p.slopes != nullptr) x -= slope2 * static_cast<float>(abs(away0 - at));
-          if (!full) {
-            const bool sees = static_cast<uint32_t>(away0 - at) < static_cast<uint32_t>(p.window) || t0 + 4 * lg + at < sq.pre;
-            x = sees ? x : -__builtin_huge_valf();
+          for (int e = 0; e < 4; ++e) {
+            const int at = 16 * h + e;
+            float y = s[x][h][e] * factor;
+            if (p.biased != 0) y -= slope2[x] * static_cast<float>(abs(away0 - at));
+            if (!full) {
+              const bool sees = static_cast<uint32_t>(away0 - at) < static_cast<uint32_t>(p.window) || t0 + 4 * lg + at < sq.pre;
+              y = sees ? y : -__builtin_huge_valf();
+            }
+            s[x][h][e] = y;
+            top = fmaxf(top, y);
           }
-          s[h][e] = x;
-          top = fmaxf(top, x);
+        top = rows_max(top);
+        if (__any(top > m_ref[x] + 8.0f)) {  // the reference follows only where a tile passes it by 2^8
+          const float m_new = fmaxf(m_ref[x], top);
+          const float alpha = __builtin_amdgcn_exp2f(m_ref[x] - (m_new == -__builtin_huge_valf() ? 0.0f : m_new));
+          m_ref[x] = m_new;
+          l_run[x] *= alpha;
+#pragma unroll
+          for (int b = 0; b < NB; ++b) acc[x][b] *= alpha;
         }
-      top = rows_max(top);
-      if (__any(top > m_ref + 8.0f)) {  // the reference follows only where a tile passes it by 2^8
-        const float m_new = fmaxf(m_ref, top);
-        const float alpha = __builtin_amdgcn_exp2f(m_ref - (m_new == -__builtin_huge_valf() ? 0.0f : m_new));
-        m_ref = m_new;
-        l_run *= alpha;
+        const float ref = m_ref[x] == -__builtin_huge_valf() ? 0.0f : m_ref[x];
 #pragma unroll
-        for (int b = 0; b < NB; ++b) acc[b] *= alpha;
-      }
-      const float ref = m_ref == -__builtin_huge_valf() ? 0.0f : m_ref;
-      // Weights as a sum of two parts of the dtype, exact to 2^-16: the products
-      // are a small part of a call that waits for memory.
-      u32x2 hi[TG], lo[TG];
+        for (int h = 0; h < TG; ++h) {
+          float w4[4];
 #pragma unroll
-      for (int h = 0; h < TG; ++h) {
-        float w4[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          w4[e] = __builtin_amdgcn_exp2f(s[h][e] - ref);
-          l_run += w4[e];
+          for (int e = 0; e < 4; ++e) {
+            w4[e] = __builtin_amdgcn_exp2f(s[x][h][e] - ref);
+            l_run[x] += w4[e];
+          }
+          hi[x][h] = u32x2{pack2<E>(w4[0], w4[1]), pack2<E>(w4[2], w4[3])};
+          lo[x][h] = u32x2{pack2<E>(w4[0] - E::lo(hi[x][h][0]), w4[1] - E::hi(hi[x][h][0])),
+                           pack2<E>(w4[2] - E::lo(hi[x][h][1]), w4[3] - E::hi(hi[x][h][1]))};
         }
-        hi[h] = u32x2{pack2<E>(w4[0], w4[1]), pack2<E>(w4[2], w4[3])};
-        lo[h] = u32x2{pack2<E>(w4[0] - E::lo(hi[h][0]), w4[1] - E::hi(hi[h][0])),
-                      pack2<E>(w4[2] - E::lo(hi[h][1]), w4[3] - E::hi(hi[h][1]))};
       }
       const uint16_t* vt = tile.v + (4 * lg + l16 / 4) * P + 4 * (l16 % 4);
 #pragma unroll
@@ -966,35 +1069,41 @@ void row_kernel(const KParams p) {
           using lds_v4i16 = __attribute__((address_space(3))) s16x4;
           const u32x2 va = __builtin_bit_cast(
               u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + 16 * h * P + 16 * b)));
-          acc[b] = E::mfma_16x16x16(va, hi[h], acc[b]);
-          acc[b] = E::mfma_16x16x16(va, lo[h], acc[b]);
-        }
-      if (mixed && __any(bad)) {
-        // As in tile_kernel: a row takes the infinities whose key has a weight there.
-        uint32_t up[CH] = {}, down[CH] = {};
-#pragma unroll 1
-        for (int j = 0; j < TT; ++j) {
-          uint32_t word = 0;
 #pragma unroll
-          for (int h = 0; h < TG; ++h)
-#pragma unroll
-            for (int x = 0; x < 2; ++x) word |= h == j / 16 && x == j % 4 / 2 ? hi[h][x] : 0u;
-          word = j % 2 != 0 ? word >> 16 : word & 0xffffu;
-          const uint32_t takes = __shfl(word, l16 + 16 * (j % 16 / 4), kWave) != 0 ? 0xffffffffu : 0u;
-#pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            up[c] |= tile.up[j][c] & takes;
-            down[c] |= tile.down[j][c] & takes;
+          for (int x = 0; x < R; ++x) {
+            acc[x][b] = E::mfma_16x16x16(va, hi[x][h], acc[x][b]);
+            acc[x][b] = E::mfma_16x16x16(va, lo[x][h], acc[x][b]);
           }
         }
+      if (__any(bad)) {
+        // As in tile_kernel: a row takes the infinities whose key has a weight there.
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-          const int u = static_cast<int>(up[b / 2] >> (16 * (b % 2) + 4 * lg));
-          const int d = static_cast<int>(down[b / 2] >> (16 * (b % 2) + 4 * lg));
+        for (int x = 0; x < R; ++x) {
+          uint32_t up[CH] = {}, down[CH] = {};
+#pragma unroll 1
+          for (int j = 0; j < TT; ++j) {
+            uint32_t word = 0;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            acc[b][e] += __int_as_float(((u << (31 - e)) >> 31) & 0x7f800000);
-            acc[b][e] -= __int_as_float(((d << (31 - e)) >> 31) & 0x7f800000);
+            for (int h = 0; h < TG; ++h)
+#pragma unroll
+              for (int y = 0; y < 2; ++y) word |= h == j / 16 && y == j % 4 / 2 ? hi[x][h][y] : 0u;
+            word = j % 2 != 0 ? word >> 16 : word & 0xffffu;
+            const uint32_t takes = __shfl(word, l16 + 16 * (j % 16 / 4), kWave) != 0 ? 0xffffffffu : 0u;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+              up[c] |= tile.up[j][c] & takes;
+              down[c] |= tile.down[j][c] & takes;
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < NB; ++b) {
+            const int u = static_cast<int>(up[b / 2] >> (16 * (b % 2) + 4 * lg));
+            const int d = static_cast<int>(down[b / 2] >> (16 * (b % 2) + 4 * lg));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              acc[x][b][e] += __int_as_float(((u << (31 - e)) >> 31) & 0x7f800000);
+              acc[x][b][e] -= __int_as_float(((d << (31 - e)) >> 31) & 0x7f800000);
+            }
           }
         }
       }
@@ -1023,7 +1132,7 @@ void row_kernel(const KParams p) {
       for (int i = 0; i < m; i += DEPTH) {
 #pragma unroll
         for (int d = 0; d < DEPTH; ++d) {
-          if (i + d < m) consume(c0 + i + d, buf[d]);
+          if (i + d < m) consume(c0 + i + d, stage(c0 + i + d, buf[d]));
           // Past the end too, from no records, so that the waits stay for the oldest tile.
           load(c0 + i + d + DEPTH, min(i + d + DEPTH, kWave - 1), i + d + DEPTH < m, buf[d]);
           __builtin_amdgcn_sched_barrier(0);
@@ -1033,26 +1142,22 @@ void row_kernel(const KParams p) {
 
     // The waves' sums to one.
     Args& b = fresh_args();
-    const float l_all = rows_sum(l_run);
+    const int head = head_of(b), g = group_of(b);
     lds_barrier();  // every wave has read its last tile
-    if (lg == 0) {
-      sm.m[wave][l16] = m_ref;
-      sm.l[wave][l16] = l_all;
-    }
-    if (l16 < w.rows) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n) *reinterpret_cast<f32x4*>(&sm.o[wave][l16 * OP + 16 * n + 4 * lg]) = acc[n];
+    for (int r = 0; r < R; ++r) {
+      const float l_all = rows_sum(l_run[r]);
+      if (lg == 0) {
+        sm.m[wave][16 * r + l16] = m_ref[r];
+        sm.l[wave][16 * r + l16] = l_all;
+      }
+      if (16 * r + l16 < w.rows) {
+#pragma unroll
+        for (int n = 0; n < NB; ++n) *reinterpret_cast<f32x4*>(&sm.o[wave][(16 * r + l16) * OP + 16 * n + 4 * lg]) = acc[r][n];
+      }
     }
     lds_barrier();
-    const bool whole = u0 == 0 && u1 == weight;
-    const int64_t slot = (static_cast<int64_t>(g + seq) * b.hkv + kv_head) * b.slot_rows;
-    if (!whole && u0 == 0 && tid == 0) {
-      int32_t* first = b.ws_first + 2 * (static_cast<int64_t>(seq) * b.hkv + kv_head);
-      first[0] = g;
-      first[1] = 1 + (weight - u1 + share - 1) / share;
-    } else if (whole && share > 0 && tid == 0) {
-      b.ws_first[2 * (static_cast<int64_t>(seq) * b.hkv + kv_head) + 1] = 0;
-    }
+    const int64_t slot = (static_cast<int64_t>(g + seq) * b.hkv + head) * b.slot_rows;
     for (int idx = tid; idx < w.rows * (D / 4); idx += kTileThreads) {
       const int r = idx / (D / 4), d = 4 * (idx % (D / 4));
       float M = sm.m[0][r];
@@ -1070,7 +1175,7 @@ void row_kernel(const KParams p) {
       if (whole) {
         const int rt = r / b.group;
         uint16_t* dst = b.out + static_cast<int64_t>(sq.first + rt) * b.o_st +
-                        static_cast<int64_t>(kv_head * b.group + r - rt * b.group) * b.o_sh + d;
+                        static_cast<int64_t>(head * b.group + r - rt * b.group) * b.o_sh + d;
         store4<E>(b, dst, L == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : O * (b.v_scale / L));
       } else {
         *reinterpret_cast<f32x4*>(b.ws + (slot + r) * D + d) = O;
@@ -1097,7 +1202,7 @@ __global__ __launch_bounds__(kTileThreads) void row_join_kernel(const KParams p)
   const int r = static_cast<int>(blockIdx.y) * kTileWaves + wave;
   const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), 0, 0);
   const int64_t rows = static_cast<int64_t>(sq.n) * p.group;
-  if (rows > kShortRows || r >= min(static_cast<int>(rows), p.slot_rows)) return;  // a tiled sequence, or no such row
+  if (rows > p.short_rows || r >= min(static_cast<int>(rows), p.slot_rows)) return;  // a tiled sequence, or no such row
   const int64_t entry = 2 * (static_cast<int64_t>(seq) * p.hkv + kv_head);
   const int g = p.ws_first[entry], count = p.ws_first[entry + 1];
   if (count == 0) return;  // written whole
@@ -1138,11 +1243,14 @@ __global__ __launch_bounds__(kTileThreads) void row_join_kernel(const KParams p)
 // How a call is cut, from what the host knows: the sizes and the bounds.
 struct Plan {
   int64_t tile_groups = 0;  // workgroups of tile_kernel; 0: every sequence has few rows
+  int split_items = 0;      // as in KParams
+  int64_t joins = 0;        // workgroups (x) of tile_join_kernel
+  int64_t tile_ws = 0;      // rows of its partial results
   int64_t row_groups = 0;   // and of row_kernel
-  int shares = 0, slot_rows = kShortRows;
+  int short_rows = 16, shares = 0, slot_rows = 32;
   int64_t slots = 0;        // row_kernel's
   int64_t ws_bytes = 0;
-  int64_t ml_at = 0, first_at = 0;  // floats from the workspace's start
+  int64_t tile_ml_at = 0, row_at = 0, ml_at = 0, first_at = 0;  // floats from the workspace's start
 };
 
 Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max_len, int window) {
@@ -1150,23 +1258,39 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
   const int group = a->num_q_heads / a->num_kv_heads;
   const int64_t hkv = a->num_kv_heads, rows = static_cast<int64_t>(a->num_tokens) * group;
   const int64_t most_rows = static_cast<int64_t>(std::min(max_query_len, a->num_tokens)) * group;
-  if (most_rows > kShortRows) {
+  // 32 rows where that takes in every sequence (speculation); beside prompts
+  // the others mostly bring one token.
+  plan.short_rows = most_rows > 16 && most_rows <= 32 && d <= kWideRows ? 32 : 16;
+  if (most_rows > plan.short_rows) {
     // At most this many row tiles: full ones, and one more a sequence, of at least 17 rows each.
-    const int64_t tiles = rows / kTileRows + std::min<int64_t>(a->num_seqs, rows / (kShortRows + 1));
+    const int64_t tiles = rows / kTileRows + std::min<int64_t>(a->num_seqs, rows / (plan.short_rows + 1));
     plan.tile_groups = tiles * hkv;
+    // Few tiles for the 256 CUs: spread (how far, the GPU decides from the lengths).
+    const int most = d <= 128 ? 512 : 256;
+    if (rows / kTileRows * hkv < most / 2) {
+      plan.split_items = most;
+      plan.joins = std::min<int64_t>(plan.tile_groups, most / 2);
+      plan.tile_groups = std::max<int64_t>(plan.tile_groups, most);
+      plan.tile_ws = static_cast<int64_t>(most) * kTileRows;
+    }
   }
   plan.row_groups = a->num_seqs * hkv;
   // Keys that a token may see, as far as the host knows.
-  const int64_t keys = a->prefix_lens != nullptr ? max_len : std::min<int64_t>(max_len, static_cast<int64_t>(window) + 16);
+  const int64_t keys = a->prefix_lens != nullptr ? max_len : std::min<int64_t>(max_len, static_cast<int64_t>(window) + 32);
   if (keys > kWholeKeys) {
     const int64_t resident = d <= 64 ? 768 : d <= 128 ? 512 : 256;  // workgroups of row_kernel on 256 CUs
     plan.shares = static_cast<int>(std::max<int64_t>(resident / hkv, 1));
     plan.row_groups = plan.shares * hkv;
-    plan.slot_rows = static_cast<int>(std::min<int64_t>(most_rows, kShortRows));
+    plan.slot_rows = static_cast<int>(std::min<int64_t>(most_rows, plan.short_rows));
     plan.slots = (plan.shares + static_cast<int64_t>(a->num_seqs)) * hkv;
-    plan.ml_at = plan.slots * plan.slot_rows * d;
+  }
+  // One workspace: the tiles' sums and their maxima, then the rows', in floats.
+  if (plan.tile_ws > 0 || plan.slots > 0) {
+    plan.tile_ml_at = plan.tile_ws * d;
+    plan.row_at = plan.tile_ml_at + plan.tile_ws * 2;
+    plan.ml_at = plan.row_at + plan.slots * plan.slot_rows * d;
     plan.first_at = plan.ml_at + plan.slots * plan.slot_rows * 2;
-    plan.ws_bytes = 4 * (plan.first_at + 2 * a->num_seqs * hkv);
+    plan.ws_bytes = 4 * (plan.first_at + (plan.slots > 0 ? 2 * a->num_seqs * hkv : 0));
   }
   return plan;
 }
@@ -1175,6 +1299,11 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
 Plan whole_plan(const dk_varlen_attn_params* a, const Plan& with) {
   Plan plan;
   plan.tile_groups = with.tile_groups;
+  if (with.split_items > 0) {
+    const int64_t group = a->num_q_heads / a->num_kv_heads, rows = a->num_tokens * group;
+    plan.tile_groups = (rows / kTileRows + std::min<int64_t>(a->num_seqs, rows / (with.short_rows + 1))) * a->num_kv_heads;
+  }
+  plan.short_rows = with.short_rows;
   plan.row_groups = static_cast<int64_t>(a->num_seqs) * a->num_kv_heads;
   return plan;
 }
@@ -1188,11 +1317,22 @@ hipError_t launch_all(const KParams& kp, const Plan& plan, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(plan.tile_groups));
     if (bs16) hipLaunchKernelGGL((tile_kernel<E, D, FP8, true>), grid, block, 0, s, kp);
     else hipLaunchKernelGGL((tile_kernel<E, D, FP8, false>), grid, block, 0, s, kp);
+    if (kp.split_items > 0) {
+      const dim3 join(static_cast<unsigned>(plan.joins), kTileRows / 16);
+      hipLaunchKernelGGL((tile_join_kernel<E, D>), join, block, 0, s, kp);
+    }
   }
   {
     const dim3 grid(static_cast<unsigned>(plan.row_groups));
-    if (bs16) hipLaunchKernelGGL((row_kernel<E, D, FP8, true>), grid, block, 0, s, kp);
-    else hipLaunchKernelGGL((row_kernel<E, D, FP8, false>), grid, block, 0, s, kp);
+    if (kp.short_rows == 16) {
+      if (bs16) hipLaunchKernelGGL((row_kernel<E, D, 1, FP8, true>), grid, block, 0, s, kp);
+      else hipLaunchKernelGGL((row_kernel<E, D, 1, FP8, false>), grid, block, 0, s, kp);
+    } else {
+      if constexpr (D <= kWideRows) {
+        if (bs16) hipLaunchKernelGGL((row_kernel<E, D, 2, FP8, true>), grid, block, 0, s, kp);
+        else hipLaunchKernelGGL((row_kernel<E, D, 2, FP8, false>), grid, block, 0, s, kp);
+      }
+    }
     if (kp.shares > 0) {
       const dim3 join(static_cast<unsigned>(kp.num_seqs * kp.hkv), static_cast<unsigned>((kp.slot_rows + 3) / 4));
       hipLaunchKernelGGL((row_join_kernel<E, D>), join, block, 0, s, kp);
@@ -1278,6 +1418,7 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
   kp.starts = a->query_start_loc;
   kp.prefix = a->prefix_lens;
   kp.slopes = a->alibi_slopes;
+  kp.biased = a->alibi_slopes != nullptr;
   kp.q_st = static_cast<int32_t>(a->q_stride_token);
   kp.q_sh = static_cast<int32_t>(a->q_stride_head);
   kp.o_st = static_cast<int32_t>(a->out_stride_token);
@@ -1305,10 +1446,15 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
   if (plan.tile_groups > 0x7fffffff || plan.row_groups > 0x7fffffff || static_cast<int64_t>(a->num_seqs) * a->num_kv_heads > 0x7fffffff)
     return fail("%s: too many sequences x heads", op);
   kp.shares = plan.shares;
+  kp.short_rows = plan.short_rows;
   kp.slot_rows = plan.slot_rows;
-  kp.ws = static_cast<float*>(workspace);
-  kp.ws_ml = kp.ws + plan.ml_at;
-  kp.ws_first = reinterpret_cast<int32_t*>(kp.ws + plan.first_at);
+  kp.split_items = plan.split_items;
+  float* ws = static_cast<float*>(workspace);
+  kp.tile_ws = ws;
+  kp.tile_ml = ws + plan.tile_ml_at;
+  kp.ws = ws + plan.row_at;
+  kp.ws_ml = ws + plan.ml_at;
+  kp.ws_first = reinterpret_cast<int32_t*>(ws + plan.first_at);
   // floor(j / b) = (j * ceil(2^k / b)) >> k for j < 2^31 with k = 31 + ceil(log2 b):
   // the factor is off by less than 1, the product by less than 2^31 <= 2^k / b.
   int k = 31;

@@ -22,6 +22,7 @@ namespace dk {
 namespace qk_norm {
 
 constexpr int kThreads = 256;
+constexpr int kFewTokens = 512;  // up to which a token's heads are spread over workgroups
 
 struct KParams {
   const int64_t* positions;
@@ -129,8 +130,199 @@ __global__ __launch_bounds__(kThreads) void norm_rotate_kernel(const KParams p) 
   for (int i = p.rot_dim + lane; i < p.d; i += kWave) store(i, E::to_float(x[i]) * inv * E::to_float(w[i]));
 }
 
+// 8 values from 16 bytes of E.
+template <typename E>
+__device__ __forceinline__ void widen(u32x4 w, float (&x)[8]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[2 * i] = E::lo(w[i]), x[2 * i + 1] = E::hi(w[i]);
+}
+
+// 4 (N = 4) or 8 entries of a table row, 16-byte (16-bit tables: 8-byte) aligned.
+template <typename E, typename CT, int N>
+__device__ __forceinline__ void table_row(const void* base, int64_t i, float* out) {
+  if constexpr (sizeof(CT) == 4) {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4*>(static_cast<const float*>(base) + i + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) out[j + e] = v[e];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 4) {
+      const u32x2 v = *reinterpret_cast<const u32x2*>(static_cast<const uint16_t*>(base) + i + j);
+      out[j] = E::lo(v[0]), out[j + 1] = E::hi(v[0]), out[j + 2] = E::lo(v[1]), out[j + 3] = E::hi(v[1]);
+    }
+  }
+}
+
+// 8 values, rounded once, to 16 bytes of E or 8 of e4m3fn.
+template <typename E, bool FP8>
+__device__ __forceinline__ void put8(void* dst, const float (&y)[8], float scale) {
+  if constexpr (FP8) {
+    uint32_t w[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      int v = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(y[4 * i], scale), e4m3_range(y[4 * i + 1], scale), 0, false);
+      v = __builtin_amdgcn_cvt_pk_fp8_f32(e4m3_range(y[4 * i + 2], scale), e4m3_range(y[4 * i + 3], scale), v, true);
+      w[i] = static_cast<uint32_t>(v);
+    }
+    *reinterpret_cast<u32x2*>(dst) = u32x2{w[0], w[1]};
+  } else {
+    *reinterpret_cast<u32x4*>(dst) =
+        u32x4{pack2<E>(y[0], y[1]), pack2<E>(y[2], y[3]), pack2<E>(y[4], y[5]), pack2<E>(y[6], y[7])};
+  }
+}
+
+// The same with 16-byte accesses. LP lanes take a head, two chunks of 8 columns
+// each that hold the two halves of 8 pairs (NeoX: a chunk of the first half of
+// the rotated columns and its partner; GPT-J, and columns past rot_dim: two
+// neighbours), so no pair crosses lanes. A workgroup takes one token, and the
+// lanes keep its cos / sin and the weights while they go through the heads.
+// Bound by memory: 16384 tokens of 32/8 heads of 128 with the cache write are
+// 403 MB.
+template <typename E, typename CT, bool NEOX, bool FP8, int LP>
+__global__ __launch_bounds__(kThreads) void norm_rotate_vec_kernel(const KParams p) {
+  constexpr int kHeads = kThreads / LP;  // side by side
+  constexpr int kElt = FP8 ? 1 : 2;      // of the cache
+  const int c = threadIdx.x % LP;
+  const int heads = p.hq + (p.v != nullptr ? 2 : 1) * p.hkv;
+  const int64_t t = blockIdx.x;
+  const int64_t pos = p.positions[t];
+  if (pos < 0 || pos >= p.max_position) return;
+  const int64_t slot = p.v != nullptr ? p.slots[t] : 0;
+  const int64_t blk = slot >= 0 ? slot / p.block_size : p.num_blocks;
+  const int64_t off = slot - blk * p.block_size;
+  const bool put_cache = p.v == nullptr || blk < p.num_blocks;
+  const bool mine = 16 * c < p.d;
+  const int half = p.rot_dim / 2;
+  // This lane's columns, and the first of its 8 pairs.
+  const bool pairs = NEOX && 8 * c < half;
+  const int col0 = pairs ? 8 * c : 16 * c;  // past the rotated ones: pairs' chunks end at rot_dim = 16 (half / 8)
+  const int col1 = pairs ? half + 8 * c : 16 * c + 8;
+  float cs[8], sn[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) cs[j] = 1.0f, sn[j] = 0.0f;
+  if (mine) {
+    const int64_t row = pos * p.table_stride;
+    if constexpr (NEOX) {
+      if (pairs) {
+        table_row<E, CT, 8>(p.table, row + 8 * c, cs);
+        table_row<E, CT, 8>(p.table, row + half + 8 * c, sn);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (16 * c + 8 * x < p.rot_dim) {
+          table_row<E, CT, 4>(p.table, row + 8 * c + 4 * x, cs + 4 * x);
+          table_row<E, CT, 4>(p.table, row + half + 8 * c + 4 * x, sn + 4 * x);
+        }
+      }
+    }
+  }
+  const int first = static_cast<int>(blockIdx.y) * kHeads + static_cast<int>(threadIdx.x) / LP;
+  for (int h = first; h < heads; h += kHeads * static_cast<int>(gridDim.y)) {
+    const bool is_q = h < p.hq, is_v = h >= p.hq + p.hkv;
+    const int kh = is_q ? h : is_v ? h - p.hq - p.hkv : h - p.hq;
+    const uint16_t* src = is_q ? p.q + t * p.q_st + kh * p.q_sh : is_v ? p.v + t * p.v_st + kh * p.v_sh : p.k + t * p.k_st + kh * p.k_sh;
+    u32x4 r0 = {0u, 0u, 0u, 0u}, r1 = {0u, 0u, 0u, 0u};
+    if (mine) {
+      r0 = *reinterpret_cast<const u32x4*>(src + col0);
+      r1 = *reinterpret_cast<const u32x4*>(src + col1);
+    }
+    float x0[8], x1[8];
+    widen<E>(r0, x0);
+    widen<E>(r1, x1);
+    float ss = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) ss += x0[j] * x0[j] + x1[j] * x1[j];
+#pragma unroll
+    for (int o = 1; o < LP; o <<= 1) ss += __shfl_xor(ss, o, kWave);
+    if (!mine || (!is_q && !put_cache)) continue;
+    if (is_v) {
+      char* dst = static_cast<char*>(p.vc) + kElt * (blk * p.vc_sb + off * p.vc_st + kh * p.vc_sh);
+      if constexpr (FP8) {
+        put8<E, true>(dst + col0, x0, p.v_scale);
+        put8<E, true>(dst + col1, x1, p.v_scale);
+      } else {
+        *reinterpret_cast<u32x4*>(dst + 2 * col0) = r0;
+        *reinterpret_cast<u32x4*>(dst + 2 * col1) = r1;
+      }
+      continue;
+    }
+    const float inv = 1.0f / __fsqrt_rn(ss / static_cast<float>(p.d) + p.eps);
+    const uint16_t* w = is_q ? p.q_w : p.k_w;
+    float w0[8], w1[8];
+    widen<E>(*reinterpret_cast<const u32x4*>(w + col0), w0);
+    widen<E>(*reinterpret_cast<const u32x4*>(w + col1), w1);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x0[j] = x0[j] * inv * w0[j];
+      x1[j] = x1[j] * inv * w1[j];
+    }
+    float y0[8], y1[8];
+    if constexpr (NEOX) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        y0[j] = x0[j] * cs[j] - x1[j] * sn[j];
+        y1[j] = x1[j] * cs[j] + x0[j] * sn[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        y0[2 * j] = x0[2 * j] * cs[j] - x0[2 * j + 1] * sn[j];
+        y0[2 * j + 1] = x0[2 * j + 1] * cs[j] + x0[2 * j] * sn[j];
+        y1[2 * j] = x1[2 * j] * cs[4 + j] - x1[2 * j + 1] * sn[4 + j];
+        y1[2 * j + 1] = x1[2 * j + 1] * cs[4 + j] + x1[2 * j] * sn[4 + j];
+      }
+    }
+    if (is_q || p.v == nullptr) {
+      uint16_t* dst = is_q ? p.q_out + t * p.qo_st + kh * p.qo_sh : p.k_out + t * p.ko_st + kh * p.ko_sh;
+      put8<E, false>(dst + col0, y0, 1.0f);
+      put8<E, false>(dst + col1, y1, 1.0f);
+    } else {
+      char* dst = static_cast<char*>(p.kc) + kElt * (blk * p.kc_sb + off * p.kc_st + kh * p.kc_sh);
+      put8<E, FP8>(dst + kElt * col0, y0, p.k_scale);
+      put8<E, FP8>(dst + kElt * col1, y1, p.k_scale);
+    }
+  }
+}
+
+// 16-byte accesses everywhere, and whole chunks on either side of rot_dim.
+template <typename CT>
+bool vectorizable(const KParams& p, bool fp8) {
+  const int half = p.rot_dim / 2;
+  auto rows = [](const void* b, int64_t st, int64_t sh) { return aligned_to(b, 16) && st % 8 == 0 && sh % 8 == 0; };
+  bool ok = p.d % 16 == 0 && p.d <= 256 && p.rot_dim % (p.neox ? 16 : 8) == 0 &&
+            (p.hq == 0 || (rows(p.q, p.q_st, p.q_sh) && rows(p.q_out, p.qo_st, p.qo_sh) && aligned_to(p.q_w, 16))) &&
+            (p.hkv == 0 || (rows(p.k, p.k_st, p.k_sh) && aligned_to(p.k_w, 16)));
+  ok = ok && (sizeof(CT) == 4 ? aligned_to(p.table, 16) && p.table_stride % 4 == 0 && half % 4 == 0
+                              : aligned_to(p.table, 8) && p.table_stride % 4 == 0 && half % 4 == 0);
+  if (p.v == nullptr) return ok && (p.hkv == 0 || rows(p.k_out, p.ko_st, p.ko_sh));
+  const int bytes = fp8 ? 8 : 16;  // of 8 elements: strides are multiples of 8 elements either way
+  return ok && rows(p.v, p.v_st, p.v_sh) && aligned_to(p.kc, bytes) && aligned_to(p.vc, bytes) && p.kc_sb % 8 == 0 &&
+         p.kc_st % 8 == 0 && p.kc_sh % 8 == 0 && p.vc_sb % 8 == 0 && p.vc_st % 8 == 0 && p.vc_sh % 8 == 0;
+}
+
+template <typename E, typename CT, bool FP8, int LP>
+hipError_t launch_vec(const KParams& kp, hipStream_t s) {
+  const int heads = kp.hq + (kp.v != nullptr ? 2 : 1) * kp.hkv;
+  const int passes = (heads + kThreads / LP - 1) / (kThreads / LP);
+  // A token's heads over several workgroups where there are few tokens.
+  const int split = kp.num_tokens <= kFewTokens ? passes : 1;
+  const dim3 grid(static_cast<unsigned>(kp.num_tokens), static_cast<unsigned>(split)), block(kThreads);
+  if (kp.neox) hipLaunchKernelGGL((norm_rotate_vec_kernel<E, CT, true, FP8, LP>), grid, block, 0, s, kp);
+  else hipLaunchKernelGGL((norm_rotate_vec_kernel<E, CT, false, FP8, LP>), grid, block, 0, s, kp);
+  return hipGetLastError();
+}
+
 template <typename E, typename CT, bool FP8>
 hipError_t launch(const KParams& kp, hipStream_t s) {
+  if (vectorizable<CT>(kp, FP8)) {
+    if (kp.d <= 64) return launch_vec<E, CT, FP8, 4>(kp, s);
+    if (kp.d <= 128) return launch_vec<E, CT, FP8, 8>(kp, s);
+    return launch_vec<E, CT, FP8, 16>(kp, s);
+  }
   const int64_t items = static_cast<int64_t>(kp.num_tokens) * (kp.hq + (kp.v != nullptr ? 2 : 1) * kp.hkv);
   const dim3 grid(static_cast<unsigned>(ceil_div64(items, kThreads / kWave))), block(kThreads);
   hipLaunchKernelGGL((norm_rotate_kernel<E, CT, FP8>), grid, block, 0, s, kp);

@@ -58,6 +58,11 @@ HIP_FLAGS = [
     f"-I{INCLUDE}",
 ]
 
+# Flags of single sources. varlen_attention.hip: matrix results in ordinary
+# registers also where a kernel has more than 256 of them; in accumulation
+# registers, its head_dim-256 sums were copied to and fro in every key tile.
+SOURCE_FLAGS = {"varlen_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+
 
 def _hipcc() -> str:
     return os.path.join(ROCM, "bin", "hipcc")
@@ -97,7 +102,7 @@ def resource_report_path(src: str) -> Path:
 def _compile_hip(src: str, resource_usage: bool) -> Path:
     BUILD.mkdir(exist_ok=True)
     obj = BUILD / (Path(src).stem + ".o")
-    cmd = [_hipcc(), RESOURCE_REMARK, *HIP_FLAGS, "-c", str(CSRC / src), "-o", str(obj)]
+    cmd = [_hipcc(), RESOURCE_REMARK, *HIP_FLAGS, *SOURCE_FLAGS.get(src, []), "-c", str(CSRC / src), "-o", str(obj)]
     out = _run(cmd, quiet_remarks=not resource_usage)
     resource_report_path(src).write_text(out)
     return obj

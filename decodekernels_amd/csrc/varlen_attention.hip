@@ -325,6 +325,11 @@ struct TileSmem {
   uint32_t up[2][TK][D / 32], down[2][TK][D / 32];
 };
 
+template <int D>
+constexpr int tile_occupancy() {  // waves per SIMD
+  return D <= 192 ? 2 : 1;
+}
+
 // Prompts: a workgroup takes 128 rows of one KV head, (token, query head of the
 // group) pairs of one sequence, 32 a wave, and all key tiles that they see (or
 // an equal part of them). Scores are formed transposed, S^T = K Q^T on
@@ -334,7 +339,7 @@ struct TileSmem {
 // operand of O^T = V^T P^T as they stand, with V^T read transposed from LDS.
 // O^T has its row in the same lane again, so rescaling is a multiplication.
 template <typename E, int D, bool FP8, bool BS16>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(D <= 128 ? 2 : 1, D <= 128 ? 2 : 1)))
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(tile_occupancy<D>(), tile_occupancy<D>())))
 void tile_kernel(const KParams p) {
   using Smem = TileSmem<D>;
   constexpr int TK = Smem::TK, KP = Smem::KP, VP = Smem::VP;
@@ -1266,7 +1271,7 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
     const int64_t tiles = rows / kTileRows + std::min<int64_t>(a->num_seqs, rows / (plan.short_rows + 1));
     plan.tile_groups = tiles * hkv;
     // Few tiles for the 256 CUs: spread (how far, the GPU decides from the lengths).
-    const int most = d <= 128 ? 512 : 256;
+    const int most = d <= 192 ? 512 : 256;
     if (rows / kTileRows * hkv < most / 2) {
       plan.split_items = most;
       plan.joins = std::min<int64_t>(plan.tile_groups, most / 2);

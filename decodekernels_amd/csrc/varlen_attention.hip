@@ -83,7 +83,6 @@ __device__ __forceinline__ f32x16 mfma_32x32x16<F16>(u32x4 a, u32x4 b, f32x16 c)
 
 constexpr int kTileWaves = 4;
 constexpr int kTileThreads = kTileWaves * kWave;
-constexpr int kTileRows = 32 * kTileWaves;  // (token, query head of the group) rows of a workgroup
 constexpr int kRsrcWord3 = 0x00020000;      // word 3 of a gfx9-family buffer resource for raw loads
 constexpr int kSeqsPerThread = 4;
 constexpr int kWholeKeys = 512;             // keys up to which a sequence of few rows is never cut
@@ -135,6 +134,11 @@ template <int D>
 constexpr int tile_keys() {
   return D <= 128 ? 64 : 32;
 }
+
+// Rows, (token, query head of the group) pairs, of a wave of tile_kernel: 32, or
+// 16 where a head is wide and the sums of 32 would leave one wave a SIMD.
+constexpr int wave_rows(int d) { return d <= 128 ? 32 : 16; }
+constexpr int tile_rows(int d) { return kTileWaves * wave_rows(d); }
 
 // Barrier for data exchanged through LDS only: global loads stay in flight.
 __device__ __forceinline__ void lds_barrier() {
@@ -195,10 +199,11 @@ __device__ __forceinline__ void store4(const Params& p, uint16_t* dst, f32x4 y) 
 }
 
 // Row tiles of a sequence: none where its few rows run in row_kernel.
+template <int D>
 __device__ __forceinline__ int row_tiles(const KParams& p, int start, int end) {
   const int first = min(max(start, 0), p.num_tokens);
   const int64_t rows = static_cast<int64_t>(max(min(end, p.num_tokens) - first, 0)) * p.group;
-  return rows > p.short_rows ? static_cast<int>((rows + kTileRows - 1) / kTileRows) : 0;
+  return rows > p.short_rows ? static_cast<int>((rows + tile_rows(D) - 1) / tile_rows(D)) : 0;
 }
 
 // Sequences s0 .. s0 + 1023, 4 a thread: weight(s) units each. Sets w and the
@@ -285,18 +290,18 @@ __device__ __forceinline__ KeyTiles key_tiles(int pre, int lo, int hi) {
 
 // A row tile of a sequence: its rows, the positions of the first and the last,
 // the keys that some row sees besides the prefix, and the key tiles that hold them.
-template <int TK>
+template <int D>
 struct RowTile {
   int row0, rows, pos0, pos1, lo, hi;
   KeyTiles tiles;
   __device__ __forceinline__ RowTile(const KParams& p, const Seq& sq, int local) {
-    row0 = local * kTileRows;
-    rows = min(sq.n * p.group - row0, kTileRows);
+    row0 = local * tile_rows(D);
+    rows = min(sq.n * p.group - row0, tile_rows(D));
     pos0 = sq.len - sq.n + row0 / p.group;
     pos1 = sq.len - sq.n + (row0 + rows - 1) / p.group;
     lo = max(pos0 - p.window + 1, 0);
     hi = max(pos1 + 1, 0);
-    tiles = key_tiles<TK>(sq.pre, lo, hi);
+    tiles = key_tiles<tile_keys<D>()>(sq.pre, lo, hi);
   }
   // Key tiles of one of `parts` parts.
   __device__ __forceinline__ int per_part(int parts) const {
@@ -314,7 +319,8 @@ template <int D>
 struct TileSmem {
   static constexpr int TK = tile_keys<D>();
   static constexpr int KP = D + 8;   // row pitches in elements: K rows 4 banks apart, for 16-byte reads of 16 rows;
-  static constexpr int VP = D + 32;  // V rows 16 banks apart, for transpose reads of 64 bytes of 4 rows
+  // V rows 16 (8) banks apart, for transpose reads of 64 (32) bytes of 4 rows
+  static constexpr int VP = D + wave_rows(D);
   struct __attribute__((aligned(16))) Stage {
     uint16_t k[TK * KP];
     uint16_t v[TK * VP];
@@ -325,27 +331,50 @@ struct TileSmem {
   uint32_t up[2][TK][D / 32], down[2][TK][D / 32];
 };
 
-template <int D>
-constexpr int tile_occupancy() {  // waves per SIMD
-  return D <= 192 ? 2 : 1;
-}
+// Prompts: a workgroup takes 128 rows (64 of wide heads) of one KV head, (token,
+// query head of the group) pairs of one sequence, 32 (16) a wave, and all key
+// tiles that they see (or an equal part of them). Scores are formed transposed,
+// S^T = K Q^T on 32x32x16 (16x16x32) MFMAs, so that a lane holds keys
+// 8 g + 4 part + i of one row, g and i its elements, part = lane / 32 (16): the
+// maximum and sum of a row need one exchange (two), and the weights are, rounded
+// to the dtype, the B operand of O^T = V^T P^T as they stand, with V^T read
+// transposed from LDS. O^T has its row in the same lane again, so rescaling is
+// a multiplication.
+template <typename E, int D>
+struct TileMath {
+  static constexpr int WR = wave_rows(D);
+  typedef float acc_t __attribute__((ext_vector_type(WR == 32 ? 16 : 4)));
+  static __device__ __forceinline__ acc_t mma(u32x4 a, u32x4 b, acc_t c) {
+    if constexpr (WR == 32) return mfma_32x32x16<E>(a, b, c);
+    else return E::mfma_16x16x32(a, b, c);
+  }
+  // Over the lanes that hold a row.
+  static __device__ __forceinline__ float row_max(float v) {
+    if constexpr (WR == 16) return rows_max(v);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+  }
+  static __device__ __forceinline__ float row_sum(float v) {
+    if constexpr (WR == 16) return rows_sum(v);
+    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(x[0]) + __uint_as_float(x[1]);
+  }
+};
 
-// Prompts: a workgroup takes 128 rows of one KV head, (token, query head of the
-// group) pairs of one sequence, 32 a wave, and all key tiles that they see (or
-// an equal part of them). Scores are formed transposed, S^T = K Q^T on
-// 32x32x16 MFMAs, so that a lane holds 16 of 32 keys of one row (row l % 32,
-// keys 8 (i / 4) + 4 (l / 32) + i % 4): the maximum and sum of a row need one
-// exchange between two lanes, and the weights are, rounded to the dtype, the B
-// operand of O^T = V^T P^T as they stand, with V^T read transposed from LDS.
-// O^T has its row in the same lane again, so rescaling is a multiplication.
 template <typename E, int D, bool FP8, bool BS16>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(tile_occupancy<D>(), tile_occupancy<D>())))
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void tile_kernel(const KParams p) {
   using Smem = TileSmem<D>;
   constexpr int TK = Smem::TK, KP = Smem::KP, VP = Smem::VP;
-  constexpr int KB = TK / 32;        // 32-key blocks of a tile
-  constexpr int NB = D / 32;         // 32-column blocks of the output
-  constexpr int KS = D / 16;         // column steps of Q.K^T
+  using Math = TileMath<E, D>;
+  using Acc = typename Math::acc_t;
+  constexpr int WR = Math::WR;
+  constexpr int NE = WR == 32 ? 16 : 4;  // elements of a lane in an accumulator
+  constexpr int KB = TK / WR;        // key blocks of a tile
+  constexpr int NB = D / WR;         // column blocks of the output
+  constexpr int CS = 8 * (kWave / WR);  // columns of a step of Q.K^T, and keys of one of P.V
+  constexpr int KS = D / CS;
+  constexpr int PS = TK / CS;
   constexpr int RW = TK / kTileWaves;  // key rows that a wave loads
   constexpr int CPR = D / 8;         // 8-element chunks of a row
   constexpr int NI = RW * CPR / kWave;
@@ -356,7 +385,7 @@ void tile_kernel(const KParams p) {
   const int tid = threadIdx.x;
   const int lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int l32 = lane % 32, half = lane / 32;
+  const int lr = lane % WR, part4 = 4 * (lane / WR);
 
   // Later tiles (long ones under a causal mask) first; the KV heads of a tile
   // next to one another, so that with 8 of them each XCD's L2 holds one head.
@@ -366,7 +395,7 @@ void tile_kernel(const KParams p) {
   // all; how many tiles there are is known only now.
   int seq, local, parts = 1;
   locate(
-      p.num_seqs, loc, [&](int s) { return row_tiles(p, p.starts[s], p.starts[s + 1]); },
+      p.num_seqs, loc, [&](int s) { return row_tiles<D>(p, p.starts[s], p.starts[s + 1]); },
       [&](int total) {
         parts = parts_of(p, total);
         return item / p.hkv / parts;
@@ -376,35 +405,35 @@ void tile_kernel(const KParams p) {
   if (seq < 0) return;
   const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), scalar_load(p.lens, seq),
                           p.prefix != nullptr ? scalar_load(p.prefix, seq) : 0);
-  const RowTile<TK> rt(p, sq, local);
+  const RowTile<D> rt(p, sq, local);
   const int row0 = rt.row0, rows = rt.rows, pos0 = rt.pos0, pos1 = rt.pos1, lo = rt.lo, hi = rt.hi;
   const KeyTiles tiles = rt.tiles;
   const int per = rt.per_part(parts);
   const int n0 = min(part * per, tiles.count), n1 = min(n0 + per, tiles.count);
   if (parts > 1 && part > 0 && n0 == n1) return;  // fewer parts than asked for
   // Positions of this wave's first and last row.
-  const int wave_row0 = min(32 * wave, rows - 1), wave_row1 = min(32 * wave + 31, rows - 1);
-  const bool wave_live = 32 * wave < rows;
+  const int wave_row0 = min(WR * wave, rows - 1), wave_row1 = min(WR * wave + WR - 1, rows - 1);
+  const bool wave_live = WR * wave < rows;
   const int wpos0 = sq.len - sq.n + (row0 + wave_row0) / p.group;
   const int wpos1 = sq.len - sq.n + (row0 + wave_row1) / p.group;
   // This lane's row; rows past the last one repeat it and are not stored.
-  const int row = row0 + min(32 * wave + l32, rows - 1);
+  const int row = row0 + min(WR * wave + lr, rows - 1);
   const int tok = row / p.group;
   const int q_head = kv_head * p.group + (row - tok * p.group);
   const int pos = sq.len - sq.n + tok;
   const int64_t token = sq.first + tok;
-  u32x4 qf[KS];  // B operand: row l32, columns 16 s + 8 half ...
+  u32x4 qf[KS];  // B operand: row lr, columns CS s + 2 part4 ...
   {
-    const uint16_t* src = p.q + token * p.q_st + static_cast<int64_t>(q_head) * p.q_sh + 8 * half;
+    const uint16_t* src = p.q + token * p.q_st + static_cast<int64_t>(q_head) * p.q_sh + 2 * part4;
     const bool wide = (reinterpret_cast<uintptr_t>(p.q) % 16 == 0) && p.q_st % 8 == 0 && p.q_sh % 8 == 0;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       if (wide) {
-        qf[s] = *reinterpret_cast<const u32x4*>(src + 16 * s);
+        qf[s] = *reinterpret_cast<const u32x4*>(src + CS * s);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          qf[s][e] = static_cast<uint32_t>(src[16 * s + 2 * e]) | static_cast<uint32_t>(src[16 * s + 2 * e + 1]) << 16;
+          qf[s][e] = static_cast<uint32_t>(src[CS * s + 2 * e]) | static_cast<uint32_t>(src[CS * s + 2 * e + 1]) << 16;
       }
 #pragma unroll
       for (int e = 0; e < 4; ++e) qf[s][e] ^= p.q_sign;
@@ -505,9 +534,9 @@ void tile_kernel(const KParams p) {
     }
   };
 
-  f32x16 acc[NB];  // O^T: row l32, columns 32 b + 8 (i / 4) + 4 half + i % 4
+  Acc acc[NB];  // O^T: row lr, columns WR b + 8 (i / 4) + part4 + i % 4
 #pragma unroll
-  for (int b = 0; b < NB; ++b) acc[b] = f32x16{};
+  for (int b = 0; b < NB; ++b) acc[b] = Acc{};
   float m_ref = -__builtin_huge_valf();  // log2 units
   float l_run = 0.0f;                    // this lane's share of the row's sum
 
@@ -516,15 +545,15 @@ void tile_kernel(const KParams p) {
     // Seen by no row of this wave / by all of them.
     if (!wave_live || (t0 >= sq.pre && (t0 > wpos1 || t0 + TK <= wpos0 - p.window + 1))) return;
     const bool full = t0 + TK <= sq.pre || (t0 + TK - 1 <= wpos0 && t0 > wpos1 - p.window);
-    f32x16 s[KB];
-    const uint16_t* kt = sm.stage[st].k + l32 * KP + 8 * half;
+    Acc s[KB];
+    const uint16_t* kt = sm.stage[st].k + lr * KP + 2 * part4;
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
-      s[b] = f32x16{};
+      s[b] = Acc{};
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
-        const u32x4 ka = *reinterpret_cast<const u32x4*>(kt + 32 * b * KP + 16 * c);
-        s[b] = mfma_32x32x16<E>(ka, qf[c], s[b]);
+        const u32x4 ka = *reinterpret_cast<const u32x4*>(kt + WR * b * KP + CS * c);
+        s[b] = Math::mma(ka, qf[c], s[b]);
       }
     }
     float factor = p.scale2;
@@ -534,28 +563,28 @@ void tile_kernel(const KParams p) {
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < NE; ++i)
           s[b][i] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][i] * p.scale2) + 1.0f);
       factor = 1.0f;
     }
     if (p.slopes != nullptr) {
-      const int away0 = fresh_vgpr(pos - t0 - 4 * half);
+      const int away0 = fresh_vgpr(pos - t0 - part4);
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          s[b][i] = s[b][i] * factor - slope2 * static_cast<float>(abs(away0 - (32 * b + 8 * (i / 4) + i % 4)));
+        for (int i = 0; i < NE; ++i)
+          s[b][i] = s[b][i] * factor - slope2 * static_cast<float>(abs(away0 - (WR * b + 8 * (i / 4) + i % 4)));
       factor = 1.0f;
     }
     if (!full) {
       // Past a prefix, key j is seen where 0 <= pos - j < window.
       // (fresh_vgpr: formed here, not 32 differences kept in registers across the tiles)
-      const int away0 = fresh_vgpr(pos - t0 - 4 * half), to_prefix = fresh_vgpr(sq.pre - t0 - 4 * half);
+      const int away0 = fresh_vgpr(pos - t0 - part4), to_prefix = fresh_vgpr(sq.pre - t0 - part4);
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int at = 32 * b + 8 * (i / 4) + i % 4;
+        for (int i = 0; i < NE; ++i) {
+          const int at = WR * b + 8 * (i / 4) + i % 4;
           const bool sees = static_cast<uint32_t>(away0 - at) < static_cast<uint32_t>(p.window) || at < to_prefix;
           s[b][i] = sees ? s[b][i] * factor : -__builtin_huge_valf();
           if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few lane masks at a time
@@ -566,11 +595,8 @@ void tile_kernel(const KParams p) {
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-    {
-      const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(top), __float_as_uint(top), false, false);
-      top = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-    }
+      for (int i = 0; i < NE; ++i) top = fmaxf(top, s[b][i]);
+    top = Math::row_max(top);
     top *= factor;
     // The reference maximum follows only when a tile passes it by 2^8.
     if (__any(top > m_ref + 8.0f)) {
@@ -581,66 +607,68 @@ void tile_kernel(const KParams p) {
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) acc[b][i] *= alpha;
+        for (int i = 0; i < NE; ++i) acc[b][i] *= alpha;
     }
     const float ref = m_ref == -__builtin_huge_valf() ? 0.0f : m_ref;  // nothing seen yet
-    u32x4 pk[2 * KB];  // B operand: row l32, 16 keys a step
+    u32x4 pk[PS];  // B operand: row lr, CS keys a step
 #pragma unroll
     for (int b = 0; b < KB; ++b)
 #pragma unroll
-      for (int i = 0; i < 16; i += 2) {
+      for (int i = 0; i < NE; i += 2) {
         const float x = __builtin_amdgcn_exp2f(s[b][i] * factor - ref);
         const float y = __builtin_amdgcn_exp2f(s[b][i + 1] * factor - ref);
         l_run += x + y;
-        pk[2 * b + i / 8][(i % 8) / 2] = pack2<E>(x, y);
+        pk[(NE * b + i) / 8][(NE * b + i) % 8 / 2] = pack2<E>(x, y);
       }
-    const uint16_t* vt = sm.stage[st].v + (4 * half + (lane % 16) / 4) * VP + 16 * ((lane / 16) % 2) + 4 * (lane % 4);
-    // A operand of O^T: columns 32 b + l32, the 16 keys of step c in the order of pk[c].
+    const uint16_t* vt =
+        sm.stage[st].v + (part4 + (lane % 16) / 4) * VP + (WR == 32 ? 16 * ((lane / 16) % 2) : 0) + 4 * (lane % 4);
+    // A operand of O^T: columns WR b + lr, the keys of step c in the order of pk[c].
     auto v_operand = [&](int c, int b) {
       using lds_v4i16 = __attribute__((address_space(3))) s16x4;
       const u32x2 x = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + 16 * c * VP + 32 * b)));
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + CS * c * VP + WR * b)));
       const u32x2 y = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + (16 * c + 8) * VP + 32 * b)));
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + (CS * c + CS / 2) * VP + WR * b)));
       return u32x4{x[0], x[1], y[0], y[1]};
     };
 #pragma unroll
-    for (int c = 0; c < 2 * KB; ++c)
+    for (int c = 0; c < PS; ++c)
 #pragma unroll
-      for (int b = 0; b < NB; ++b) acc[b] = mfma_32x32x16<E>(v_operand(c, b), pk[c], acc[b]);
+      for (int b = 0; b < NB; ++b) acc[b] = Math::mma(v_operand(c, b), pk[c], acc[b]);
     if (all_see(t0)) return;
     int bad = 0;
 #pragma unroll
     for (int w = 0; w < kTileWaves; ++w) bad |= sm.bad[st][w];
     if (__builtin_amdgcn_readfirstlane(bad) == 0) return;
     // Infinities and NaN among values that not every row sees: a row takes
-    // those whose key has a weight there (0 x infinity would be NaN). Key
-    // 8 (e / 4) + 4 half + e % 4 of a 16-key step is element e of its half.
-    uint32_t up[NB] = {}, down[NB] = {};
+    // those whose key has a weight there (0 x infinity would be NaN).
+    uint32_t up[D / 32] = {}, down[D / 32] = {};
 #pragma unroll 1
     for (int j = 0; j < TK; ++j) {
       if (__builtin_amdgcn_readfirstlane(sm.bad[st][j / RW]) == 0) continue;
-      const int e = j % 4 + 4 * ((j % 16) / 8);
+      // Key j is element `at` of the lanes of part (j % WR / 4) % (64 / WR).
+      const int at = NE * (j / WR) + 4 * (j % WR / (kWave / WR * 4)) + j % 4;
       uint32_t word = 0;
 #pragma unroll
-      for (int c = 0; c < 2 * KB; ++c) {
-        if (c != j / 16) continue;
+      for (int c = 0; c < PS; ++c) {
+        if (c != at / 8) continue;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) word |= w == e / 2 ? pk[c][w] : 0u;
+        for (int w = 0; w < 4; ++w) word |= w == at % 8 / 2 ? pk[c][w] : 0u;
       }
-      word = e % 2 != 0 ? word >> 16 : word & 0xffffu;
-      const uint32_t takes = __shfl(word, l32 + 32 * ((j / 4) % 2), kWave) != 0 ? 0xffffffffu : 0u;
+      word = at % 2 != 0 ? word >> 16 : word & 0xffffu;
+      const uint32_t takes = __shfl(word, lr + WR * (j / 4 % (kWave / WR)), kWave) != 0 ? 0xffffffffu : 0u;
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
+      for (int b = 0; b < D / 32; ++b) {
         up[b] |= sm.up[st][j][b] & takes;
         down[b] |= sm.down[st][j][b] & takes;
       }
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
-      const int u = static_cast<int>(up[b] >> (4 * half)), d = static_cast<int>(down[b] >> (4 * half));
+      const int u = static_cast<int>(up[WR * b / 32] >> (part4 + WR * b % 32));
+      const int d = static_cast<int>(down[WR * b / 32] >> (part4 + WR * b % 32));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < NE; ++i) {
         constexpr int kInf = 0x7f800000;
         const int at = 31 - (8 * (i / 4) + i % 4);
         acc[b][i] += __int_as_float(((u << at) >> 31) & kInf);
@@ -663,38 +691,34 @@ void tile_kernel(const KParams p) {
     }
   }
 
-  {
-    const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(l_run), __float_as_uint(l_run), false, false);
-    l_run = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-  }
-  if (32 * wave + l32 >= rows) return;
+  l_run = Math::row_sum(l_run);
+  if (WR * wave + lr >= rows) return;
   if (parts > 1) {
     // Partial results: sums against m_ref, joined by tile_join_kernel.
-    const int64_t slot = (static_cast<int64_t>(item) * kTileRows) + 32 * wave + l32;
-    float* dst = p.tile_ws + slot * D;
-    if (half == 0) {
+    const int64_t slot = static_cast<int64_t>(item) * tile_rows(D) + WR * wave + lr;
+    float* dst = p.tile_ws + slot * D + part4;
+    if (part4 == 0) {
       p.tile_ml[2 * slot] = m_ref;
       p.tile_ml[2 * slot + 1] = l_run;
     }
 #pragma unroll
     for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int g = 0; g < 4; ++g)
-        *reinterpret_cast<f32x4*>(dst + 32 * b + 8 * g + 4 * half) =
+      for (int g = 0; g < NE / 4; ++g)
+        *reinterpret_cast<f32x4*>(dst + WR * b + 8 * g) =
             f32x4{acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
     return;
   }
   const float inv = l_run == 0.0f ? 0.0f : p.v_scale / l_run;
-  uint16_t* dst = p.out + token * p.o_st + static_cast<int64_t>(q_head) * p.o_sh + 4 * half;
+  uint16_t* dst = p.out + token * p.o_st + static_cast<int64_t>(q_head) * p.o_sh + part4;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < NE / 4; ++g) {
       const f32x4 y = {acc[b][4 * g], acc[b][4 * g + 1], acc[b][4 * g + 2], acc[b][4 * g + 3]};
-      store4<E>(p, dst + 32 * b + 8 * g, l_run == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : y * inv);
+      store4<E>(p, dst + WR * b + 8 * g, l_run == 0.0f ? f32x4{0.f, 0.f, 0.f, 0.f} : y * inv);
     }
 }
-
 
 // Joins the parts of row tiles over which tile_kernel was spread, in their
 // order. Workgroup (x, y) takes 16 rows of tile x / hkv, KV head x % hkv.
@@ -707,7 +731,7 @@ __global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams p
   const int kv_head = static_cast<int>(blockIdx.x) % p.hkv;
   const int item0 = static_cast<int>(blockIdx.x) / p.hkv;
   locate(
-      p.num_seqs, loc, [&](int s) { return row_tiles(p, p.starts[s], p.starts[s + 1]); },
+      p.num_seqs, loc, [&](int s) { return row_tiles<D>(p, p.starts[s], p.starts[s + 1]); },
       [&](int total) {
         parts = parts_of(p, total);
         return item0;
@@ -716,7 +740,7 @@ __global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams p
   if (seq < 0 || parts == 1) return;
   const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), scalar_load(p.lens, seq),
                           p.prefix != nullptr ? scalar_load(p.prefix, seq) : 0);
-  const RowTile<tile_keys<D>()> rt(p, sq, local);
+  const RowTile<D> rt(p, sq, local);
   const int per = rt.per_part(parts);
   const int used = max((rt.tiles.count + per - 1) / per, 1);
   const int d = 4 * (static_cast<int>(threadIdx.x) % LD);
@@ -724,8 +748,8 @@ __global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams p
        r < min(16 * static_cast<int>(blockIdx.y) + 16, rt.rows); r += RS) {
     if (static_cast<int>(threadIdx.x) >= RS * LD) break;
     // Part i's item is (item0 parts + i) hkv + the KV head, counted from the last (tile_kernel).
-    const int64_t slot = (static_cast<int64_t>(item0) * parts * p.hkv + (p.hkv - 1 - kv_head)) * kTileRows + r;
-    const int64_t step = static_cast<int64_t>(p.hkv) * kTileRows;
+    const int64_t slot = (static_cast<int64_t>(item0) * parts * p.hkv + (p.hkv - 1 - kv_head)) * tile_rows(D) + r;
+    const int64_t step = static_cast<int64_t>(p.hkv) * tile_rows(D);
     float M = -__builtin_huge_valf();
 #pragma unroll 4
     for (int i = 0; i < used; ++i) M = fmaxf(M, p.tile_ml[2 * (slot + i * step)]);
@@ -1268,15 +1292,15 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
   plan.short_rows = most_rows > 16 && most_rows <= 32 && d <= kWideRows ? 32 : 16;
   if (most_rows > plan.short_rows) {
     // At most this many row tiles: full ones, and one more a sequence, of at least 17 rows each.
-    const int64_t tiles = rows / kTileRows + std::min<int64_t>(a->num_seqs, rows / (plan.short_rows + 1));
+    const int64_t tiles = rows / tile_rows(d) + std::min<int64_t>(a->num_seqs, rows / (plan.short_rows + 1));
     plan.tile_groups = tiles * hkv;
     // Few tiles for the 256 CUs: spread (how far, the GPU decides from the lengths).
-    const int most = d <= 192 ? 512 : 256;
-    if (rows / kTileRows * hkv < most / 2) {
+    constexpr int most = 512;
+    if (rows / tile_rows(d) * hkv < most / 2) {
       plan.split_items = most;
       plan.joins = std::min<int64_t>(plan.tile_groups, most / 2);
       plan.tile_groups = std::max<int64_t>(plan.tile_groups, most);
-      plan.tile_ws = static_cast<int64_t>(most) * kTileRows;
+      plan.tile_ws = static_cast<int64_t>(most) * tile_rows(d);
     }
   }
   plan.row_groups = a->num_seqs * hkv;
@@ -1301,12 +1325,12 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
 }
 
 // The plan without a workspace: nothing is cut.
-Plan whole_plan(const dk_varlen_attn_params* a, const Plan& with) {
+Plan whole_plan(const dk_varlen_attn_params* a, int d, const Plan& with) {
   Plan plan;
   plan.tile_groups = with.tile_groups;
   if (with.split_items > 0) {
     const int64_t group = a->num_q_heads / a->num_kv_heads, rows = a->num_tokens * group;
-    plan.tile_groups = (rows / kTileRows + std::min<int64_t>(a->num_seqs, rows / (with.short_rows + 1))) * a->num_kv_heads;
+    plan.tile_groups = (rows / tile_rows(d) + std::min<int64_t>(a->num_seqs, rows / (with.short_rows + 1))) * a->num_kv_heads;
   }
   plan.short_rows = with.short_rows;
   plan.row_groups = static_cast<int64_t>(a->num_seqs) * a->num_kv_heads;
@@ -1323,7 +1347,7 @@ hipError_t launch_all(const KParams& kp, const Plan& plan, hipStream_t s) {
     if (bs16) hipLaunchKernelGGL((tile_kernel<E, D, FP8, true>), grid, block, 0, s, kp);
     else hipLaunchKernelGGL((tile_kernel<E, D, FP8, false>), grid, block, 0, s, kp);
     if (kp.split_items > 0) {
-      const dim3 join(static_cast<unsigned>(plan.joins), kTileRows / 16);
+      const dim3 join(static_cast<unsigned>(plan.joins), tile_rows(D) / 16);
       hipLaunchKernelGGL((tile_join_kernel<E, D>), join, block, 0, s, kp);
     }
   }
@@ -1446,7 +1470,7 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
   kp.v_scale = v_scale;
   kp.hkv = a->num_kv_heads;
   Plan plan = make_plan(a, head_dim, max_query_len, max_len, kp.window);
-  if (plan.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < plan.ws_bytes)) plan = whole_plan(a, plan);
+  if (plan.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < plan.ws_bytes)) plan = whole_plan(a, head_dim, plan);
   if (plan.ws_bytes > 0 && !aligned_to(workspace, 16)) return fail("%s: workspace must be 16-byte aligned", op);
   if (plan.tile_groups > 0x7fffffff || plan.row_groups > 0x7fffffff || static_cast<int64_t>(a->num_seqs) * a->num_kv_heads > 0x7fffffff)
     return fail("%s: too many sequences x heads", op);

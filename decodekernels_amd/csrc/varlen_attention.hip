@@ -58,14 +58,22 @@ struct KParams {
   uint32_t q_sign;
 };
 
-// 8 e4m3fn bytes as 8 elements of E, exactly.
+// 8 e4m3fn bytes as 8 elements of E, exactly (scale 1; every e4m3fn value is
+// one of E).
 template <typename E>
 __device__ __forceinline__ u32x4 fp8x8_to(u32x2 w) {
-  const auto a = __builtin_amdgcn_cvt_pk_f32_fp8(w[0], false);
-  const auto b = __builtin_amdgcn_cvt_pk_f32_fp8(w[0], true);
-  const auto c = __builtin_amdgcn_cvt_pk_f32_fp8(w[1], false);
-  const auto d = __builtin_amdgcn_cvt_pk_f32_fp8(w[1], true);
-  return u32x4{pack2<E>(a[0], a[1]), pack2<E>(b[0], b[1]), pack2<E>(c[0], c[1]), pack2<E>(d[0], d[1])};
+  u32x4 out;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (std::is_same<E, Bf16>::value) {
+      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.0f, false));
+      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[i], 1.0f, true));
+    } else {
+      out[2 * i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, false));
+      out[2 * i + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w[i], 1.0f, true));
+    }
+  }
+  return out;
 }
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -86,6 +94,7 @@ constexpr int kTileThreads = kTileWaves * kWave;
 constexpr int kRsrcWord3 = 0x00020000;      // word 3 of a gfx9-family buffer resource for raw loads
 constexpr int kSeqsPerThread = 4;
 constexpr int kWholeKeys = 512;             // keys up to which a sequence of few rows is never cut
+constexpr int kMorePart = 8;                // key tiles by which a part may grow for the sake of one piece a workgroup
 constexpr int kMinPart = 8;                 // key tiles of a part of a row tile at least
 constexpr int kWideRows = 192;              // head_dim up to which row_kernel takes 32 rows: 256 has no registers for them
 constexpr int kMinShare = 16;               // key tiles a workgroup of row_kernel takes at least
@@ -206,19 +215,14 @@ __device__ __forceinline__ int row_tiles(const KParams& p, int start, int end) {
   return rows > p.short_rows ? static_cast<int>((rows + tile_rows(D) - 1) / tile_rows(D)) : 0;
 }
 
-// Sequences s0 .. s0 + 1023, 4 a thread: weight(s) units each. Sets w and the
-// units before each of them (from `base` on) and returns the units in all.
-template <typename Weight>
-__device__ __forceinline__ int scan_sequences(int num_seqs, int s0, int base, LocateSmem& sm, Weight weight,
-                                              int (&w)[kSeqsPerThread], int (&before)[kSeqsPerThread]) {
+// Prefix sums over sequences, 4 a thread: of the thread's units w, from `base`
+// on, to `before`; returns the units in all.
+__device__ __forceinline__ int scan_units(int base, LocateSmem& sm, const int (&w)[kSeqsPerThread],
+                                          int (&before)[kSeqsPerThread]) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const int s = s0 + tid * kSeqsPerThread;
   int sum = 0;
 #pragma unroll
-  for (int i = 0; i < kSeqsPerThread; ++i) {
-    w[i] = s + i < num_seqs ? weight(s + i) : 0;
-    sum += w[i];
-  }
+  for (int i = 0; i < kSeqsPerThread; ++i) sum += w[i];
   int scan = sum;
 #pragma unroll
   for (int off = 1; off < kWave; off <<= 1) {
@@ -243,32 +247,48 @@ __device__ __forceinline__ int scan_sequences(int num_seqs, int s0, int base, Lo
   return __builtin_amdgcn_readfirstlane(total);
 }
 
-// Units of all sequences; then, with target(total), the sequence and the unit
-// of it that hold this one of them (seq = -1: it is past them).
-template <typename Weight, typename Target>
-__device__ __forceinline__ int locate(int num_seqs, LocateSmem& sm, Weight weight, Target target, int& seq, int& local) {
+// weight(s) units a sequence; plan(total) is then told how many there are, and
+// says whether units(w) parts of a sequence are counted instead of its w units.
+// target() names one of them: the sequence that holds it and which one of the
+// sequence's it is (seq = -1: past the last).
+template <typename Weight, typename PlanFn, typename Units, typename Target>
+__device__ __forceinline__ void locate(int num_seqs, LocateSmem& sm, Weight weight, PlanFn plan, Units units,
+                                       Target target, int& seq, int& local) {
   constexpr int kStep = kTileThreads * kSeqsPerThread;
-  const int last = (num_seqs - 1) / kStep * kStep;
+  const int mine = static_cast<int>(threadIdx.x) * kSeqsPerThread;
+  const bool one = num_seqs <= kStep;  // one step: the units stay in registers
   int w[kSeqsPerThread], before[kSeqsPerThread];
+  auto load = [&](int s0) {
+#pragma unroll
+    for (int i = 0; i < kSeqsPerThread; ++i) w[i] = s0 + mine + i < num_seqs ? weight(s0 + mine + i) : 0;
+  };
   int total = 0;
-  for (int s0 = 0; s0 < num_seqs; s0 += kStep) total += scan_sequences(num_seqs, s0, total, sm, weight, w, before);
-  const int want = target(total);
+  for (int s0 = 0; s0 < num_seqs; s0 += kStep) {
+    load(s0);
+    total += scan_units(total, sm, w, before);
+  }
+  const bool parts = plan(total);
+  const int want = target();
   int base = 0;
-  for (int s0 = last > 0 ? 0 : last; s0 < num_seqs; s0 += kStep) {
-    if (last > 0) base += scan_sequences(num_seqs, s0, base, sm, weight, w, before);  // else w and before still hold
+  for (int s0 = 0; s0 < num_seqs; s0 += kStep) {
+    if (!one) load(s0);
+    if (parts) {
+#pragma unroll
+      for (int i = 0; i < kSeqsPerThread; ++i) w[i] = units(w[i]);
+    }
+    if (!one || parts) base += scan_units(base, sm, w, before);  // else `before` still holds
 #pragma unroll
     for (int i = 0; i < kSeqsPerThread; ++i) {
       if (want >= before[i] && want < before[i] + w[i]) {
-        sm.seq = s0 + static_cast<int>(threadIdx.x) * kSeqsPerThread + i;
+        sm.seq = s0 + mine + i;
         sm.local = want - before[i];
       }
     }
-    if (last > 0 && want < base) break;
+    if (!one && want < base) break;
   }
   lds_barrier();
   seq = __builtin_amdgcn_readfirstlane(sm.seq);
   local = __builtin_amdgcn_readfirstlane(sm.local);
-  return total;
 }
 
 // The key tiles that some row of a workgroup sees: those of the prefix, then
@@ -398,9 +418,9 @@ void tile_kernel(const KParams p) {
       p.num_seqs, loc, [&](int s) { return row_tiles<D>(p, p.starts[s], p.starts[s + 1]); },
       [&](int total) {
         parts = parts_of(p, total);
-        return item / p.hkv / parts;
+        return false;
       },
-      seq, local);
+      [](int w) { return w; }, [&] { return item / p.hkv / parts; }, seq, local);
   const int part = item / p.hkv % parts;
   if (seq < 0) return;
   const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), scalar_load(p.lens, seq),
@@ -734,9 +754,9 @@ __global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams p
       p.num_seqs, loc, [&](int s) { return row_tiles<D>(p, p.starts[s], p.starts[s + 1]); },
       [&](int total) {
         parts = parts_of(p, total);
-        return item0;
+        return false;
       },
-      seq, local);
+      [](int w) { return w; }, [&] { return item0; }, seq, local);
   if (seq < 0 || parts == 1) return;
   const Seq sq = make_seq(p, scalar_load(p.starts, seq), scalar_load(p.starts, seq + 1), scalar_load(p.lens, seq),
                           p.prefix != nullptr ? scalar_load(p.prefix, seq) : 0);
@@ -843,6 +863,7 @@ void row_kernel(const KParams p) {
   auto weight_of = [&](const Work& w) { return w.rows > 0 ? max(w.tiles.count, 1) : 0; };
 
   int seq, local, share = 0;
+  bool single = false;
   if (Args& a = fresh_args(); a.shares > 0) {
     locate(
         a.num_seqs, sm.loc,
@@ -851,8 +872,20 @@ void row_kernel(const KParams p) {
         },
         [&](int all) {
           share = max((all + a.shares - 1) / a.shares, kMinShare);
-          return static_cast<int>(min(static_cast<int64_t>(group_of(a)) * share, static_cast<int64_t>(all)));
+          if (a.num_seqs >= a.shares) return false;
+          // One piece a workgroup, equal parts of one sequence, where the parts
+          // get only a little longer by it.
+          // (share >= all / (shares - seqs + 1): the parts, of up to share - 1 more
+          // units each than they hold, are shares at most.)
+          const int most = a.shares - a.num_seqs + 1;
+          const int longer = max((all + most - 1) / most, kMinShare);
+          if (longer - share > kMorePart) return false;
+          share = longer;
+          single = true;
+          return true;
         },
+        [&](int units) { return (units + share - 1) / share; },
+        [&] { return single ? group_of(a) : static_cast<int>(min(static_cast<int64_t>(group_of(a)) * share, int64_t{0x7fffffff})); },
         seq, local);
     if (seq < 0) return;
   } else {
@@ -877,13 +910,19 @@ void row_kernel(const KParams p) {
       if (share == 0) return;
       continue;
     }
+    if (single) {  // part `local` of this sequence
+      const int parts = (weight + share - 1) / share;
+      left = (weight + parts - 1) / parts;
+      local = min(local * left, weight);
+    }
     const int u0 = local, u1 = share > 0 ? min(weight, local + left) : weight;
+    const int per = left;
     left -= u1 - u0;
     const bool whole = u0 == 0 && u1 == weight;
     if (share > 0 && u0 == 0 && tid == 0) {  // for row_join_kernel: the first of its pieces' workgroups, and how many
       int32_t* first = a.ws_first + 2 * (static_cast<int64_t>(seq) * a.hkv + kv_head);
       first[0] = group_of(a);
-      first[1] = whole ? 0 : 1 + (weight - u1 + share - 1) / share;
+      first[1] = whole ? 0 : single ? (weight + per - 1) / per : 1 + (weight - u1 + share - 1) / share;
     }
     // This lane's rows (the last one from there on).
     int q_head[R], pos[R];
@@ -949,20 +988,20 @@ void row_kernel(const KParams p) {
           const char* vt = vbase + ELT * (pg * p.v_sb + static_cast<int64_t>(off) * p.v_st);
           const auto brk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kt), 0, nrec, kRsrcWord3);
           const auto brv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vt), 0, nrec, kRsrcWord3);
+          auto fetch = [&](const __amdgpu_buffer_rsrc_t rsrc, int stride, u32x4* to) {
 #pragma unroll
-          for (int x = 0; x < NI; ++x) {
-            const int o = 1024 * x + 16 * lane;
-            int ko = o / RB * p.k_st * ELT + o % RB;
-            if (!inner && !used(r0 + o / RB)) ko = -1;  // past num_records: zeros
-            r.k[NI * h + x] = __builtin_amdgcn_raw_buffer_load_b128(brk, ko, 0, 2);
-          }
-#pragma unroll
-          for (int x = 0; x < NI; ++x) {
-            const int o = 1024 * x + 16 * lane;
-            int vo = o / RB * p.v_st * ELT + o % RB;
-            if (!inner && !used(r0 + o / RB)) vo = -1;
-            r.v[NI * h + x] = __builtin_amdgcn_raw_buffer_load_b128(brv, vo, 0, 2);
-          }
+            for (int x = 0; x < NI; ++x) {
+              // 1 KB of rows end to end: with whole rows, one offset a lane and scalar steps.
+              constexpr bool kStep = 1024 % RB == 0 && D < 256;  // (256: no scalar registers left for them)
+              const int o = (kStep ? 0 : 1024 * x) + 16 * lane;
+              const int step = kStep ? x * (1024 / RB) * stride * ELT : 0;
+              int off = o / RB * stride * ELT + o % RB;
+              if (!inner && !used(r0 + (1024 * x + 16 * lane) / RB)) off = -1;  // past num_records: zeros
+              to[x] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, step, 2);
+            }
+          };
+          fetch(brk, p.k_st, r.k + NI * h);
+          fetch(brv, p.v_st, r.v + NI * h);
         } else {
 #pragma unroll
           for (int x = 0; x < NI; ++x) {
@@ -1037,8 +1076,10 @@ void row_kernel(const KParams p) {
           for (int x = 0; x < R; ++x) s[x][h] = E::mfma_16x16x32(ka, qf[x][c], s[x][h]);
         }
       }
-      // Weights as a sum of two parts of the dtype, exact to 2^-16: the products
-      // are a small part of a call that waits for memory.
+      // 16-bit caches: weights as a sum of two parts of the dtype, exact to 2^-16,
+      // since the products are a small part of a call that waits for memory. An
+      // fp8 cache brings twice the keys in that time: its weights are rounded
+      // once, as in tile_kernel.
       u32x2 hi[R][TG], lo[R][TG];
 #pragma unroll
       for (int x = 0; x < R; ++x) {
@@ -1086,24 +1127,37 @@ void row_kernel(const KParams p) {
             l_run[x] += w4[e];
           }
           hi[x][h] = u32x2{pack2<E>(w4[0], w4[1]), pack2<E>(w4[2], w4[3])};
-          lo[x][h] = u32x2{pack2<E>(w4[0] - E::lo(hi[x][h][0]), w4[1] - E::hi(hi[x][h][0])),
-                           pack2<E>(w4[2] - E::lo(hi[x][h][1]), w4[3] - E::hi(hi[x][h][1]))};
+          if constexpr (!FP8)
+            lo[x][h] = u32x2{pack2<E>(w4[0] - E::lo(hi[x][h][0]), w4[1] - E::hi(hi[x][h][0])),
+                             pack2<E>(w4[2] - E::lo(hi[x][h][1]), w4[3] - E::hi(hi[x][h][1]))};
         }
       }
       const uint16_t* vt = tile.v + (4 * lg + l16 / 4) * P + 4 * (l16 % 4);
-#pragma unroll
-      for (int h = 0; h < TG; ++h)
+      using lds_v4i16 = __attribute__((address_space(3))) s16x4;
+      auto v_read = [&](int h, int b) {  // columns 16 b + l16, keys 16 h + 4 lg ...
+        return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + 16 * h * P + 16 * b)));
+      };
+      if constexpr (FP8) {
+        // 32 keys a product, in the order in which a lane has their weights.
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
-          using lds_v4i16 = __attribute__((address_space(3))) s16x4;
-          const u32x2 va = __builtin_bit_cast(
-              u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + 16 * h * P + 16 * b)));
+          const u32x2 v0 = v_read(0, b), v1 = v_read(1, b);
+#pragma unroll
+          for (int x = 0; x < R; ++x)
+            acc[x][b] = E::mfma_16x16x32(u32x4{v0[0], v0[1], v1[0], v1[1]},
+                                         u32x4{hi[x][0][0], hi[x][0][1], hi[x][1][0], hi[x][1][1]}, acc[x][b]);
+        }
+      } else {
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+          const u32x2 va = v_read(0, b);
 #pragma unroll
           for (int x = 0; x < R; ++x) {
-            acc[x][b] = E::mfma_16x16x16(va, hi[x][h], acc[x][b]);
-            acc[x][b] = E::mfma_16x16x16(va, lo[x][h], acc[x][b]);
+            acc[x][b] = E::mfma_16x16x16(va, hi[x][0], acc[x][b]);
+            acc[x][b] = E::mfma_16x16x16(va, lo[x][0], acc[x][b]);
           }
         }
+      }
       if (__any(bad)) {
         // As in tile_kernel: a row takes the infinities whose key has a weight there.
 #pragma unroll
@@ -1214,7 +1268,7 @@ void row_kernel(const KParams p) {
         }
       }
     }
-    if (left <= 0) return;
+    if (single || left <= 0) return;
     lds_barrier();  // the sums have been read: the next piece's tiles may take their place
   }
 }

@@ -41,6 +41,8 @@ struct KParams {
   int hkv;
   int split_items;         // tile_kernel: workgroups that the tiles of a call may be split over; 0: never split
   int shares;              // row_kernel: workgroups a KV head, of equal shares of all key tiles; 0: one a sequence
+  int tile_groups;         // workgroups of tile_work
+  int row_from;            // the first workgroup of row_work
   int short_rows;          // rows of a KV head up to which a sequence runs in row_kernel: 16 or 32
   int slot_rows;           // row_kernel: rows of a slot, as many as max_query_len allows
   // Partial results, row by row of an item or slot: sums, and their reference
@@ -57,6 +59,16 @@ struct KParams {
   float cap2, scale2;
   uint32_t q_sign;
 };
+
+// The kernel's arguments, to be loaded where they are used: an argument that
+// the compiler sees only here does not stay in scalar registers around it.
+// KParams is the one parameter, at the start of the argument segment.
+typedef const __attribute__((address_space(4))) KParams Args;
+__device__ __forceinline__ Args& fresh_args() {
+  auto a = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
+  __asm__ volatile("" : "+s"(a));
+  return *a;
+}
 
 // 8 e4m3fn bytes as 8 elements of E, exactly (scale 1; every e4m3fn value is
 // one of E).
@@ -156,16 +168,6 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-// The kernel's arguments, to be loaded where they are used: an argument that
-// the compiler sees only here does not stay in scalar registers around it.
-// KParams is the one parameter, at the start of the argument segment.
-typedef const __attribute__((address_space(4))) KParams Args;
-__device__ __forceinline__ Args& fresh_args() {
-  auto a = (Args*)__builtin_amdgcn_kernarg_segment_ptr();
-  __asm__ volatile("" : "+s"(a));
-  return *a;
-}
-
 // A uniform int32 through the scalar cache (data of earlier kernels only).
 __device__ __forceinline__ int scalar_load(const int32_t* base, int64_t i) {
   return ((const __attribute__((address_space(4))) int32_t*)base)[i];
@@ -209,7 +211,7 @@ __device__ __forceinline__ void store4(const Params& p, uint16_t* dst, f32x4 y) 
 
 // Row tiles of a sequence: none where its few rows run in row_kernel.
 template <int D>
-__device__ __forceinline__ int row_tiles(const KParams& p, int start, int end) {
+__device__ __forceinline__ int row_tiles(Args& p, int start, int end) {
   const int first = min(max(start, 0), p.num_tokens);
   const int64_t rows = static_cast<int64_t>(max(min(end, p.num_tokens) - first, 0)) * p.group;
   return rows > p.short_rows ? static_cast<int>((rows + tile_rows(D) - 1) / tile_rows(D)) : 0;
@@ -314,7 +316,7 @@ template <int D>
 struct RowTile {
   int row0, rows, pos0, pos1, lo, hi;
   KeyTiles tiles;
-  __device__ __forceinline__ RowTile(const KParams& p, const Seq& sq, int local) {
+  __device__ __forceinline__ RowTile(Args& p, const Seq& sq, int local) {
     row0 = local * tile_rows(D);
     rows = min(sq.n * p.group - row0, tile_rows(D));
     pos0 = sq.len - sq.n + row0 / p.group;
@@ -331,7 +333,7 @@ struct RowTile {
 
 // Workgroups over which the key tiles of a row tile are spread, so that all
 // make up to split_items.
-__device__ __forceinline__ int parts_of(const KParams& p, int total) {
+__device__ __forceinline__ int parts_of(Args& p, int total) {
   return p.split_items > 0 && total > 0 ? max(p.split_items / (total * p.hkv), 1) : 1;
 }
 
@@ -349,6 +351,7 @@ struct TileSmem {
   // any, and then a bit for each column (infinity or NaN; minus infinity or NaN).
   int bad[2][kTileWaves];
   uint32_t up[2][TK][D / 32], down[2][TK][D / 32];
+  LocateSmem loc;
 };
 
 // Prompts: a workgroup takes 128 rows (64 of wide heads) of one KV head, (token,
@@ -382,8 +385,7 @@ struct TileMath {
 };
 
 template <typename E, int D, bool FP8, bool BS16>
-__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void tile_kernel(const KParams p) {
+__device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
   using Smem = TileSmem<D>;
   constexpr int TK = Smem::TK, KP = Smem::KP, VP = Smem::VP;
   using Math = TileMath<E, D>;
@@ -400,8 +402,6 @@ void tile_kernel(const KParams p) {
   constexpr int NI = RW * CPR / kWave;
   constexpr int ELT = FP8 ? 1 : 2;
   using Chunk = typename std::conditional<FP8, u32x2, u32x4>::type;
-  __shared__ Smem sm;
-  __shared__ LocateSmem loc;
   const int tid = threadIdx.x;
   const int lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
@@ -409,13 +409,13 @@ void tile_kernel(const KParams p) {
 
   // Later tiles (long ones under a causal mask) first; the KV heads of a tile
   // next to one another, so that with 8 of them each XCD's L2 holds one head.
-  const int item = static_cast<int>(gridDim.x) - 1 - static_cast<int>(blockIdx.x);
+  const int item = p.tile_groups - 1 - static_cast<int>(blockIdx.x);
   const int kv_head = p.hkv - 1 - item % p.hkv;
   // With few tiles each goes over as many workgroups as make split_items in
   // all; how many tiles there are is known only now.
   int seq, local, parts = 1;
   locate(
-      p.num_seqs, loc, [&](int s) { return row_tiles<D>(p, p.starts[s], p.starts[s + 1]); },
+      p.num_seqs, sm.loc, [&](int s) { return row_tiles<D>(p, p.starts[s], p.starts[s + 1]); },
       [&](int total) {
         parts = parts_of(p, total);
         return false;
@@ -750,10 +750,18 @@ void tile_kernel(const KParams p) {
     }
 }
 
+// The workgroups of tile_work alone (wide heads; the others share a launch with row_work).
+template <typename E, int D, bool FP8, bool BS16>
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void tile_kernel(const KParams) {
+  __shared__ TileSmem<D> sm;
+  tile_work<E, D, FP8, BS16>(fresh_args(), sm);
+}
+
 // Joins the parts of row tiles over which tile_kernel was spread, in their
 // order. Workgroup (x, y) takes 16 rows of tile x / hkv, KV head x % hkv.
 template <typename E, int D>
-__global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams p) {
+__global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams) {
+  Args& p = fresh_args();
   constexpr int LD = D / 4;                  // lanes of a row
   constexpr int RS = kTileThreads / LD;      // rows side by side
   __shared__ LocateSmem loc;
@@ -832,10 +840,8 @@ constexpr int row_occupancy() {  // waves per SIMD
 // not a whole sequence leaves its sums in slot g + s (sequence s; no two pieces
 // share one) for row_join_kernel. Scores are S^T = K Q^T and the output O^T =
 // V^T P^T on 16x16 MFMAs: lane l holds rows l % 16 (and + 16) of both.
-template <typename E, int D, int R, bool FP8, bool BS16>
-__global__ __launch_bounds__(kTileThreads)
-__attribute__((amdgpu_waves_per_eu(row_occupancy<D, R>(), row_occupancy<D, R>())))
-void row_kernel(const KParams p) {
+template <typename E, int D, int R, bool FP8, bool BS16, typename Params>
+__device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm) {
   using Smem = RowSmem<D, R, FP8>;
   constexpr int TT = Smem::TT, P = Smem::P, OP = Smem::OP;
   constexpr int TG = TT / 16;           // 16-key groups of a tile: each lies in one cache block (BS16)
@@ -844,14 +850,13 @@ void row_kernel(const KParams p) {
   constexpr int RB = D * ELT;           // bytes of a K (or V) row
   constexpr int NI = 16 * RB / 1024;    // 16-byte loads of a lane for a group of K (or V)
   constexpr int DEPTH = 2;              // tiles in flight
-  __shared__ Smem sm;
   const int tid = threadIdx.x;
   const int lane = tid % kWave;
   const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
   const int l16 = lane % 16, lg = lane / 16;
   // Workgroup g of a KV head (formed where they are used, as the arguments).
-  auto head_of = [](Args& x) { return static_cast<int>(blockIdx.x) % x.hkv; };
-  auto group_of = [](Args& x) { return static_cast<int>(blockIdx.x) / x.hkv; };
+  auto head_of = [](Args& x) { return (static_cast<int>(blockIdx.x) - x.row_from) % x.hkv; };
+  auto group_of = [](Args& x) { return (static_cast<int>(blockIdx.x) - x.row_from) / x.hkv; };
 
   struct Work {
     Seq sq;
@@ -1283,6 +1288,26 @@ void row_kernel(const KParams p) {
   }
 }
 
+template <typename E, int D, int R, bool FP8, bool BS16>
+__global__ __launch_bounds__(kTileThreads)
+__attribute__((amdgpu_waves_per_eu(row_occupancy<D, R>(), row_occupancy<D, R>())))
+void row_kernel(const KParams p) {
+  __shared__ RowSmem<D, R, FP8> sm;
+  row_work<E, D, R, FP8, BS16>(p, sm);
+}
+
+// Both in one launch: the tiles' workgroups, then the rows', which run beside
+// the last tiles. (Up to head_dim 128: the others need all registers for the rows.)
+template <typename E, int D, bool FP8, bool BS16>
+__global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2, 2))) void mixed_kernel(const KParams) {
+  constexpr size_t kBytes = std::max(sizeof(TileSmem<D>), sizeof(RowSmem<D, 1, FP8>));
+  __shared__ __attribute__((aligned(16))) char raw[kBytes];
+  if (static_cast<int>(blockIdx.x) < fresh_args().tile_groups)
+    tile_work<E, D, FP8, BS16>(fresh_args(), *reinterpret_cast<TileSmem<D>*>(raw));
+  else
+    row_work<E, D, 1, FP8, BS16>(fresh_args(), *reinterpret_cast<RowSmem<D, 1, FP8>*>(raw));
+}
+
 // Joins the pieces of row_kernel's cut sequences, in their order: a wave a row.
 template <typename E, int D>
 __global__ __launch_bounds__(kTileThreads) void row_join_kernel(const KParams p) {
@@ -1351,6 +1376,8 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
   const int group = a->num_q_heads / a->num_kv_heads;
   const int64_t hkv = a->num_kv_heads, rows = static_cast<int64_t>(a->num_tokens) * group;
   const int64_t most_rows = static_cast<int64_t>(std::min(max_query_len, a->num_tokens)) * group;
+  // Keys that a token may see, as far as the host knows.
+  const int64_t keys = a->prefix_lens != nullptr ? max_len : std::min<int64_t>(max_len, static_cast<int64_t>(window) + std::max(max_query_len, 32));
   // 32 rows where that takes in every sequence (speculation); beside prompts
   // the others mostly bring one token.
   plan.short_rows = most_rows > 16 && most_rows <= 32 && d <= kWideRows ? 32 : 16;
@@ -1360,7 +1387,7 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
     plan.tile_groups = tiles * hkv;
     // Few tiles for the 256 CUs: spread (how far, the GPU decides from the lengths).
     constexpr int most = 512;
-    if (rows / tile_rows(d) * hkv < most / 2) {
+    if (rows / tile_rows(d) * hkv < most / 2 && keys > kMinPart * (d <= 128 ? tile_keys<128>() : tile_keys<256>())) {
       plan.split_items = most;
       plan.joins = std::min<int64_t>(plan.tile_groups, most / 2);
       plan.tile_groups = std::max<int64_t>(plan.tile_groups, most);
@@ -1368,8 +1395,6 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
     }
   }
   plan.row_groups = a->num_seqs * hkv;
-  // Keys that a token may see, as far as the host knows.
-  const int64_t keys = a->prefix_lens != nullptr ? max_len : std::min<int64_t>(max_len, static_cast<int64_t>(window) + 32);
   if (keys > kWholeKeys) {
     const int64_t resident = d <= 64 ? 768 : d <= 128 ? 512 : 256;  // workgroups of row_kernel on 256 CUs
     plan.shares = static_cast<int>(std::max<int64_t>(resident / hkv, 1));
@@ -1402,34 +1427,41 @@ Plan whole_plan(const dk_varlen_attn_params* a, int d, const Plan& with) {
 }
 
 template <typename E, int D, bool FP8>
-hipError_t launch_all(const KParams& kp, const Plan& plan, hipStream_t s) {
+hipError_t launch_all(KParams kp, const Plan& plan, hipStream_t s) {
   const dim3 block(kTileThreads);
   // Rows of a 16-key group within the 2^31 bytes of a buffer resource.
   const bool bs16 = kp.block_size % 16 == 0 && int64_t{16} * 2 * std::max(kp.k_st, kp.v_st) < (int64_t{1} << 31);
-  if (plan.tile_groups > 0) {
-    const dim3 grid(static_cast<unsigned>(plan.tile_groups));
-    if (bs16) hipLaunchKernelGGL((tile_kernel<E, D, FP8, true>), grid, block, 0, s, kp);
-    else hipLaunchKernelGGL((tile_kernel<E, D, FP8, false>), grid, block, 0, s, kp);
-    if (kp.split_items > 0) {
-      const dim3 join(static_cast<unsigned>(plan.joins), tile_rows(D) / 16);
-      hipLaunchKernelGGL((tile_join_kernel<E, D>), join, block, 0, s, kp);
+  const unsigned tiles = static_cast<unsigned>(plan.tile_groups), rows = static_cast<unsigned>(plan.row_groups);
+  if (D <= 128 && tiles > 0) {
+    if constexpr (D <= 128) {
+      kp.row_from = kp.tile_groups;
+      if (bs16) hipLaunchKernelGGL((mixed_kernel<E, D, FP8, true>), dim3(tiles + rows), block, 0, s, kp);
+      else hipLaunchKernelGGL((mixed_kernel<E, D, FP8, false>), dim3(tiles + rows), block, 0, s, kp);
     }
-  }
-  {
-    const dim3 grid(static_cast<unsigned>(plan.row_groups));
-    if (kp.short_rows == 16) {
-      if (bs16) hipLaunchKernelGGL((row_kernel<E, D, 1, FP8, true>), grid, block, 0, s, kp);
-      else hipLaunchKernelGGL((row_kernel<E, D, 1, FP8, false>), grid, block, 0, s, kp);
-    } else {
-      if constexpr (D <= kWideRows) {
-        if (bs16) hipLaunchKernelGGL((row_kernel<E, D, 2, FP8, true>), grid, block, 0, s, kp);
-        else hipLaunchKernelGGL((row_kernel<E, D, 2, FP8, false>), grid, block, 0, s, kp);
+  } else {
+    if constexpr (D > 128) {
+      if (tiles > 0) {
+        if (bs16) hipLaunchKernelGGL((tile_kernel<E, D, FP8, true>), dim3(tiles), block, 0, s, kp);
+        else hipLaunchKernelGGL((tile_kernel<E, D, FP8, false>), dim3(tiles), block, 0, s, kp);
       }
     }
-    if (kp.shares > 0) {
-      const dim3 join(static_cast<unsigned>(kp.num_seqs * kp.hkv), static_cast<unsigned>((kp.slot_rows + 3) / 4));
-      hipLaunchKernelGGL((row_join_kernel<E, D>), join, block, 0, s, kp);
+    if (kp.short_rows == 16) {
+      if (bs16) hipLaunchKernelGGL((row_kernel<E, D, 1, FP8, true>), dim3(rows), block, 0, s, kp);
+      else hipLaunchKernelGGL((row_kernel<E, D, 1, FP8, false>), dim3(rows), block, 0, s, kp);
+    } else {
+      if constexpr (D <= kWideRows) {
+        if (bs16) hipLaunchKernelGGL((row_kernel<E, D, 2, FP8, true>), dim3(rows), block, 0, s, kp);
+        else hipLaunchKernelGGL((row_kernel<E, D, 2, FP8, false>), dim3(rows), block, 0, s, kp);
+      }
     }
+  }
+  if (kp.split_items > 0) {
+    const dim3 join(static_cast<unsigned>(plan.joins), tile_rows(D) / 16);
+    hipLaunchKernelGGL((tile_join_kernel<E, D>), join, block, 0, s, kp);
+  }
+  if (kp.shares > 0) {
+    const dim3 join(static_cast<unsigned>(kp.num_seqs * kp.hkv), static_cast<unsigned>((kp.slot_rows + 3) / 4));
+    hipLaunchKernelGGL((row_join_kernel<E, D>), join, block, 0, s, kp);
   }
   return hipGetLastError();
 }
@@ -1536,8 +1568,9 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
   Plan plan = make_plan(a, head_dim, max_query_len, max_len, kp.window);
   if (plan.ws_bytes > 0 && (workspace == nullptr || workspace_bytes < plan.ws_bytes)) plan = whole_plan(a, head_dim, plan);
   if (plan.ws_bytes > 0 && !aligned_to(workspace, 16)) return fail("%s: workspace must be 16-byte aligned", op);
-  if (plan.tile_groups > 0x7fffffff || plan.row_groups > 0x7fffffff || static_cast<int64_t>(a->num_seqs) * a->num_kv_heads > 0x7fffffff)
+  if (plan.tile_groups + plan.row_groups > 0x7fffffff || static_cast<int64_t>(a->num_seqs) * a->num_kv_heads > 0x7fffffff)
     return fail("%s: too many sequences x heads", op);
+  kp.tile_groups = static_cast<int>(plan.tile_groups);
   kp.shares = plan.shares;
   kp.short_rows = plan.short_rows;
   kp.slot_rows = plan.slot_rows;

@@ -161,6 +161,13 @@ constexpr int tile_keys() {
 constexpr int wave_rows(int d) { return d <= 128 ? 32 : 16; }
 constexpr int tile_rows(int d) { return kTileWaves * wave_rows(d); }
 
+// All ones where key j lies in [0, pre) or [lo, hi), else 0. (By sign bits:
+// comparisons would put a lane mask into scalar registers for every load, and
+// short cuts branches that wait for the loads before them.)
+__device__ __forceinline__ int in_ranges(int j, int pre, int lo, int hi) {
+  return ((j - pre) | ((lo - 1 - j) & (j - hi))) >> 31;
+}
+
 // Barrier for data exchanged through LDS only: global loads stay in flight.
 __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
@@ -470,13 +477,13 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
   const char* vbase = static_cast<const char*>(p.v) + ELT * (static_cast<int64_t>(kv_head) * p.v_sh);
   const int64_t table_row = static_cast<int64_t>(seq) * p.bt_stride;
   // A key that some row of the workgroup sees.
-  auto used = [&](int j) { return j < sq.pre || (j >= lo && j < hi); };
+  auto used = [&](int j) { return in_ranges(j, sq.pre, lo, hi); };
   auto page_of = [&](int t) { return min(max(t, 0), p.num_blocks - 1); };
 
   auto load = [&](int n) {
     const int t0 = tiles.index(n) * TK;
     const int r0 = t0 + RW * wave;
-    const bool inner = t0 + TK <= sq.pre || (t0 >= lo && t0 + TK <= hi);
+    const int all = t0 + TK <= sq.pre || (t0 >= lo && t0 + TK <= hi) ? -1 : 0;  // every key of the tile
     if constexpr (BS16) {
       // The wave's rows lie in one cache block: one scalar table entry, one
       // resource each for K and V. Rows that no one sees read as zeros.
@@ -490,11 +497,16 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
       const int nrec = any ? 0x7fffffff : 0;
       const auto brk = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(kt), 0, nrec, kRsrcWord3);
       const auto brv = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(vt), 0, nrec, kRsrcWord3);
+      int hide[NI] = {};  // -1 (past num_records: zeros) for rows that no one sees
+      if (all == 0) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i) hide[i] = ~used(r0 + chunk_row(i));
+      }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        int ko = ELT * (chunk_row(i) * p.k_st + chunk_col(i));
-        int vo = ELT * (chunk_row(i) * p.v_st + chunk_col(i));
-        if (!inner && !used(r0 + chunk_row(i))) ko = vo = -1;  // past num_records
+        const int ko = hide[i] | ELT * (chunk_row(i) * p.k_st + chunk_col(i));
+        const int vo = hide[i] | ELT * (chunk_row(i) * p.v_st + chunk_col(i));
+
         if constexpr (FP8) {
           rk[i] = __builtin_amdgcn_raw_buffer_load_b64(brk, ko, 0, 0);
           rv[i] = __builtin_amdgcn_raw_buffer_load_b64(brv, vo, 0, 0);
@@ -508,7 +520,7 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
       for (int i = 0; i < NI; ++i) {
         const int j = r0 + chunk_row(i);
         rk[i] = rv[i] = Chunk{};
-        if (used(j)) {
+        if (used(j) != 0) {
           const int blk = div_block(p, j);
           const int64_t page = page_of(p.tables[table_row + blk]);
           const int64_t off = j - blk * p.block_size;
@@ -966,7 +978,7 @@ __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm
       }
       slope2[r] = a.slopes != nullptr ? a.slopes[q_head[r]] * kLog2e : 0.0f;
     }
-    auto used = [&](int j) { return j < sq.pre || (j >= w.lo && j < sq.len); };
+    auto used = [&](int j) { return in_ranges(j, sq.pre, w.lo, sq.len); };
     auto page_at = [&](auto& c, int j) {
       return min(max(c.tables[static_cast<int64_t>(seq) * c.bt_stride + div_block(c, j)], 0), c.num_blocks - 1);
     };
@@ -990,7 +1002,7 @@ __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm
     auto tile_at = [&](int i) { return w.tiles.index(u0 + wave + kTileWaves * i) * TT; };
     auto load = [&](int i, int e, bool live, Regs& r) {
       const int t0 = tile_at(i);
-      const bool inner = t0 + TT <= sq.pre || (t0 >= w.lo && t0 + TT <= sq.len);
+      const int all = t0 + TT <= sq.pre || (t0 >= w.lo && t0 + TT <= sq.len) ? -1 : 0;  // every key of the tile
 #pragma unroll
       for (int h = 0; h < TG; ++h) {
         const int r0 = t0 + 16 * h;
@@ -1011,7 +1023,7 @@ __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm
               const int o = (kStep ? 0 : 1024 * x) + 16 * lane;
               const int step = kStep ? x * (1024 / RB) * stride * ELT : 0;
               int off = o / RB * stride * ELT + o % RB;
-              if (!inner && !used(r0 + (1024 * x + 16 * lane) / RB)) off = -1;  // past num_records: zeros
+              off |= ~(all | used(r0 + (1024 * x + 16 * lane) / RB));  // -1, past num_records: zeros
               to[x] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, off, step, 2);
             }
           };
@@ -1023,7 +1035,7 @@ __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm
             const int o = 1024 * x + 16 * lane;
             const int j = r0 + o / RB;
             r.k[NI * h + x] = r.v[NI * h + x] = u32x4{0u, 0u, 0u, 0u};
-            if (live && used(j)) {
+            if (live && used(j) != 0) {
               const int blk = div_block(p, j);
               const int64_t page = page_at(p, j);
               const int64_t off = j - blk * p.block_size;
@@ -1107,23 +1119,33 @@ __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm
               s[x][h][e] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[x][h][e] * p.scale2) + 1.0f);
           factor = 1.0f;
         }
-        const int away0 = pos[x] - t0 - 4 * lg;
+        if (p.biased != 0) {
+          const int away0 = fresh_vgpr(pos[x] - t0 - 4 * lg);
+#pragma unroll
+          for (int h = 0; h < TG; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[x][h][e] = s[x][h][e] * factor - slope2[x] * static_cast<float>(abs(away0 - 16 * h - e));
+          factor = 1.0f;
+        }
+        if (!full) {
+          const int away0 = fresh_vgpr(pos[x] - t0 - 4 * lg), to_prefix = fresh_vgpr(sq.pre - t0 - 4 * lg);
+#pragma unroll
+          for (int h = 0; h < TG; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const bool sees =
+                  static_cast<uint32_t>(away0 - 16 * h - e) < static_cast<uint32_t>(p.window) || 16 * h + e < to_prefix;
+              s[x][h][e] = sees ? s[x][h][e] * factor : -__builtin_huge_valf();
+            }
+          factor = 1.0f;
+        }
         float top = -__builtin_huge_valf();
 #pragma unroll
         for (int h = 0; h < TG; ++h)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int at = 16 * h + e;
-            float y = s[x][h][e] * factor;
-            if (p.biased != 0) y -= slope2[x] * static_cast<float>(abs(away0 - at));
-            if (!full) {
-              const bool sees = static_cast<uint32_t>(away0 - at) < static_cast<uint32_t>(p.window) || t0 + 4 * lg + at < sq.pre;
-              y = sees ? y : -__builtin_huge_valf();
-            }
-            s[x][h][e] = y;
-            top = fmaxf(top, y);
-          }
-        top = rows_max(top);
+          for (int e = 0; e < 4; ++e) top = fmaxf(top, s[x][h][e]);
+        top = rows_max(top) * factor;
         if (__any(top > m_ref[x] + 8.0f)) {  // the reference follows only where a tile passes it by 2^8
           const float m_new = fmaxf(m_ref[x], top);
           const float alpha = __builtin_amdgcn_exp2f(m_ref[x] - (m_new == -__builtin_huge_valf() ? 0.0f : m_new));
@@ -1138,7 +1160,7 @@ __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm
           float w4[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            w4[e] = __builtin_amdgcn_exp2f(s[x][h][e] - ref);
+            w4[e] = __builtin_amdgcn_exp2f(s[x][h][e] * factor - ref);
             l_run[x] += w4[e];
           }
           hi[x][h] = u32x2{pack2<E>(w4[0], w4[1]), pack2<E>(w4[2], w4[3])};

@@ -39,7 +39,7 @@ INCLUDE = ROOT / "include"
 BUILD = PKG / "_build"
 
 HIP_SOURCES = ["capi.hip", "paged_attention.hip", "gemm.hip", "norm_act.hip", "rope_cache.hip", "noalloc_scratch.hip",
-               "slot_mapping.hip", "qk_norm_rope.hip", "varlen_attention.hip"]
+               "slot_mapping.hip", "qk_norm_rope.hip", "varlen_attention.hip", "varlen_attention_f16.hip"]
 LIB_NAME = "libdecodekernels_amd.so"
 EXT_NAME = "_C.so"
 ARCH = "gfx950"
@@ -58,10 +58,11 @@ HIP_FLAGS = [
     f"-I{INCLUDE}",
 ]
 
-# Flags of single sources. varlen_attention.hip: matrix results in ordinary
+# Flags of single sources. The varlen attention's: matrix results in ordinary
 # registers also where a kernel has more than 256 of them; in accumulation
 # registers, its head_dim-256 sums were copied to and fro in every key tile.
-SOURCE_FLAGS = {"varlen_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+_VGPR_FORM = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+SOURCE_FLAGS = {"varlen_attention.hip": _VGPR_FORM, "varlen_attention_f16.hip": _VGPR_FORM}
 
 
 def _hipcc() -> str:

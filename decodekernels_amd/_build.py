@@ -83,7 +83,7 @@ def _run(cmd: list[str], quiet_remarks: bool = False) -> str:
     if quiet_remarks:  # drop each resource remark and the source excerpt under it
         kept, skip = [], False
         for line in out.splitlines():
-            if RESOURCE_REMARK in line:
+            if RESOURCE_REMARK in line or line.startswith("In file included from"):
                 skip = True
             elif skip and "|" in line[:12]:
                 pass

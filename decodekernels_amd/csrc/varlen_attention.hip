@@ -31,7 +31,8 @@ Plan make_plan(const dk_varlen_attn_params* a, int d, int max_query_len, int max
     }
   }
   plan.row_groups = a->num_seqs * hkv;
-  if (keys > kWholeKeys) {
+  const bool many = a->num_seqs * hkv >= kManyPairs;
+  if (keys > (many ? kWholeKeysMany : kWholeKeys)) {
     const int64_t resident = d <= 64 ? 768 : d <= 128 ? 512 : 256;  // workgroups of row_kernel on 256 CUs
     plan.shares = static_cast<int>(std::max<int64_t>(resident / hkv, 1));
     plan.row_groups = plan.shares * hkv;
@@ -168,6 +169,7 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
   kp.q_sign = c < 0.0f ? 0x80008000u : 0u;
   kp.cap2 = a->softcap * kLog2e;
   kp.scale2 = std::fabs(c) * kLog2e * (a->softcap > 0.0f ? 2.0f / a->softcap : 1.0f);
+  if (!(kp.scale2 < INFINITY)) return fail("%s: scale / softcap is past fp32's range", op);
   hipStream_t s = static_cast<hipStream_t>(stream);
   return static_cast<int>(dtype == DK_BFLOAT16 ? launch<Bf16>(kp, plan, head_dim, fp8, s)
                                                : launch<F16>(kp, plan, head_dim, fp8, s));
@@ -179,7 +181,9 @@ int run(const char* op, const dk_varlen_attn_params* a, int dtype, int head_dim,
 extern "C" int64_t dk_paged_attention_varlen_workspace_bytes(const dk_varlen_attn_params* a, int head_dim,
                                                              int max_query_len, int max_seq_len) {
   using namespace dk::varlen;
-  if (a == nullptr || a->num_kv_heads <= 0 || a->num_q_heads < a->num_kv_heads || a->num_tokens <= 0 || a->num_seqs <= 0 ||
+  if (a == nullptr || a->num_kv_heads <= 0 || a->num_q_heads < a->num_kv_heads ||
+      a->num_q_heads % a->num_kv_heads != 0 || a->num_q_heads / a->num_kv_heads > DK_MAX_GQA_GROUP || head_dim > 256 ||
+      a->num_tokens <= 0 || a->num_seqs <= 0 ||
       max_query_len < 0 || max_seq_len < 0 || a->num_blocks < 0 || a->max_blocks < 0 || a->block_size <= 0 || head_dim <= 0)
     return 0;  // nothing to do, or refused by the call
   const int max_len = length_bound(a, max_seq_len);

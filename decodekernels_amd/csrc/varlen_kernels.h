@@ -107,11 +107,19 @@ constexpr int kTileWaves = 4;
 constexpr int kTileThreads = kTileWaves * kWave;
 constexpr int kRsrcWord3 = 0x00020000;      // word 3 of a gfx9-family buffer resource for raw loads
 constexpr int kSeqsPerThread = 4;
-constexpr int kWholeKeys = 512;             // keys up to which a sequence of few rows is never cut
-constexpr int kMorePart = 8;                // key tiles by which a part may grow for the sake of one piece a workgroup
-constexpr int kMinPart = 8;                 // key tiles of a part of a row tile at least
-constexpr int kWideRows = 192;              // head_dim up to which row_kernel takes 32 rows: 256 has no registers for them
-constexpr int kMinShare = 16;               // key tiles a workgroup of row_kernel takes at least
+// Sequences of few rows are not cut up to so many keys: the joining launch costs
+// more than it gives. Nor up to kWholeKeysMany where kManyPairs (sequence, KV
+// head) pairs fill the CUs by themselves: 32 sequences of 100-900 keys, 8 KV
+// heads, 31.7 us cut and 25.2 whole (cold); 29 of 1-1800 keys 36.4 and 33.3.
+constexpr int kWholeKeys = 512, kWholeKeysMany = 2048, kManyPairs = 192;
+// Key tiles that a workgroup takes at least (7 pairs x 2 heads of 71-569 keys,
+// head_dim 256: 25.2 us with 16, 21.9 with 8), and by which an equal part of a
+// sequence may be longer than an equal share of all, for the sake of one piece a
+// workgroup (48 speculating sequences of 200-8000 keys: 66.8 us with 8, 62.5 with
+// 32; twice the share is too many: 32 sequences of 500-8000 keys 105 and 134 us).
+constexpr int kMinShare = 8, kMorePart = 32;
+constexpr int kMinPart = 8;     // key tiles of a part of a row tile at least
+constexpr int kWideRows = 192;  // head_dim up to which 32 rows share a reading: 256 has no registers for them
 
 // Infinities and NaN of the dtype: the exponent bits of an element, and the
 // lowest of them.
@@ -158,8 +166,9 @@ constexpr int tile_keys() {
   return D <= 128 ? 64 : 32;
 }
 
-// Rows, (token, query head of the group) pairs, of a wave of tile_kernel: 32, or
-// 16 where a head is wide and the sums of 32 would leave one wave a SIMD.
+// Rows, (token, query head of the group) pairs, of a wave of tile_work: 32, or
+// 16 where a head is wide and the sums of 32 would leave one wave a SIMD (nine
+// ragged prompts, head_dim 256: 376 us with 32 rows, 286 with 16).
 constexpr int wave_rows(int d) { return d <= 128 ? 32 : 16; }
 constexpr int tile_rows(int d) { return kTileWaves * wave_rows(d); }
 
@@ -185,6 +194,20 @@ __device__ __forceinline__ int scalar_load(const int32_t* base, int64_t i) {
 template <typename Params>
 __device__ __forceinline__ int div_block(const Params& p, int j) {
   return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(j)) * p.bs_mul) >> p.bs_shift);
+}
+
+// cap tanh(y) in log2 units, for a product q.k: tanh y = 1 - 2 / (e^(2 y) + 1)
+// has the right ends and an absolute error of some 2^-23, a few 1e-5 of a score
+// under caps up to kExactCap. Larger ones take tanh's series where |y| < 0.1.
+constexpr float kExactCap = 64.0f;
+template <bool LARGE, typename Params>
+__device__ __forceinline__ float capped(const Params& p, float product) {
+  const float z = product * p.scale2;  // 2 y log2 e
+  const float t = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(z) + 1.0f);
+  if constexpr (!LARGE) return t;
+  const float y = z * (0.5f / kLog2e), y2 = y * y;
+  const float series = p.cap2 * y * (1.0f + y2 * (-1.0f / 3.0f + y2 * (2.0f / 15.0f - y2 * (17.0f / 315.0f))));
+  return fabsf(y) < 0.1f ? series : t;
 }
 
 // What a sequence brings to this call.
@@ -218,7 +241,7 @@ __device__ __forceinline__ void store4(const Params& p, uint16_t* dst, f32x4 y) 
   }
 }
 
-// Row tiles of a sequence: none where its few rows run in row_kernel.
+// Row tiles of a sequence: none where its few rows run in row_work.
 template <int D>
 __device__ __forceinline__ int row_tiles(Args& p, int start, int end) {
   const int first = min(max(start, 0), p.num_tokens);
@@ -508,7 +531,6 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
       for (int i = 0; i < NI; ++i) {
         const int ko = hide[i] | ELT * (chunk_row(i) * p.k_st + chunk_col(i));
         const int vo = hide[i] | ELT * (chunk_row(i) * p.v_st + chunk_col(i));
-
         if constexpr (FP8) {
           rk[i] = __builtin_amdgcn_raw_buffer_load_b64(brk, ko, 0, 0);
           rv[i] = __builtin_amdgcn_raw_buffer_load_b64(brv, vo, 0, 0);
@@ -602,13 +624,17 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
     __builtin_amdgcn_sched_group_barrier(0x8, 8, 0);
     float factor = p.scale2;
     if (p.cap2 > 0.0f) {
-      // tanh y = 1 - 2 / (e^(2y) + 1): -1 and 1 at the ends, absolute error of
-      // an fp32 step of 1 near 0.
+      if (p.cap2 <= kExactCap * kLog2e) {
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
+        for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int i = 0; i < NE; ++i)
-          s[b][i] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[b][i] * p.scale2) + 1.0f);
+          for (int i = 0; i < NE; ++i) s[b][i] = capped<false>(p, s[b][i]);
+      } else {
+#pragma unroll
+        for (int b = 0; b < KB; ++b)
+#pragma unroll
+          for (int i = 0; i < NE; ++i) s[b][i] = capped<true>(p, s[b][i]);
+      }
       factor = 1.0f;
     }
     if (p.slopes != nullptr) {
@@ -1108,17 +1134,23 @@ __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm
       // 16-bit caches: weights as a sum of two parts of the dtype, exact to 2^-16,
       // since the products are a small part of a call that waits for memory. An
       // fp8 cache brings twice the keys in that time: its weights are rounded
-      // once, as in tile_kernel.
+      // once, as in tile_work.
       u32x2 hi[R][TG], lo[R][TG];
 #pragma unroll
       for (int x = 0; x < R; ++x) {
         float factor = p.scale2;
         if (p.cap2 > 0.0f) {
+          if (p.cap2 <= kExactCap * kLog2e) {
 #pragma unroll
-          for (int h = 0; h < TG; ++h)
+            for (int h = 0; h < TG; ++h)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[x][h][e] = p.cap2 - 2.0f * p.cap2 * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s[x][h][e] * p.scale2) + 1.0f);
+              for (int e = 0; e < 4; ++e) s[x][h][e] = capped<false>(p, s[x][h][e]);
+          } else {
+#pragma unroll
+            for (int h = 0; h < TG; ++h)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) s[x][h][e] = capped<true>(p, s[x][h][e]);
+          }
           factor = 1.0f;
         }
         if (p.biased != 0) {

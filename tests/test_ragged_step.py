@@ -19,10 +19,13 @@ relative to the value:
   relative: 2^-13 sum(p |v|).
 """
 
+import ctypes
+
 import pytest
 import torch
 
 import decodekernels_amd as dk
+from decodekernels_amd import capi
 from oracle import ragged_step as oracle
 
 pytestmark = pytest.mark.gpu
@@ -483,6 +486,125 @@ def test_attention_extreme_scores():
     b.check(b.run(scale=1.0, softcap=30.0), scale=1.0, softcap=30.0)
     b.check(b.run(scale=-0.2), scale=-0.2)
     b.check(b.run(scale=0.0), scale=0.0)  # the mean
+
+
+@pytest.mark.parametrize("cap", [0.5, 50.0, 64.0, 65.0, 1e3, 1e4, 1e8])
+def test_attention_caps_small_and_large(cap):
+    b = Batch([1, 70], [300, 400], 4, 2, 128, dtype=FP16, q_scale=4.0)
+    b.check(b.run(softcap=cap), softcap=cap)
+
+
+def test_attention_of_an_empty_cache():
+    q = torch.randn(3, 4, 64, device=DEV).to(BF16)
+    cache = torch.empty(0, 16, 2, 64, dtype=BF16, device=DEV)
+    for columns in (0, 2):
+        tables = torch.zeros(2, columns, dtype=torch.int32, device=DEV)
+        out = dk.paged_attention_varlen(q, cache, cache, tables, int32([5, 5]), int32([0, 1, 3]), out=torch.ones_like(q))
+        assert not out.any()
+    b = Batch([1], [9], 4, 2, 64)
+    assert not dk.paged_attention_varlen(b.q, b.k, b.v, b.tables, int32([9]), int32([0, 1]), max_seq_len=0).any()
+    assert dk.paged_attention_varlen(q[:0], b.k, b.v, b.tables, int32([9]), int32([0, 0])).shape == (0, 4, 64)
+
+
+def test_attention_reads_every_e4m3_value():
+    """V of all 254 e4m3fn numbers, each attended to alone (window 1), and q.K
+    of a unit query with them."""
+    codes = torch.tensor([c for c in range(256) if c % 128 != 127], dtype=torch.uint8)
+    n = codes.numel()
+    for dtype in (BF16, FP16):
+        for new in ([1] * n, [n]):  # one token each, and a prompt
+            seqs = len(new)
+            v = codes.to(DEV).view(FP8)
+            cache = torch.zeros(n, 1, 1, 64, dtype=torch.uint8, device=DEV).view(FP8)
+            cache.view(torch.uint8)[:] = codes.to(DEV)[:, None, None, None]
+            tables = torch.arange(n, dtype=torch.int32, device=DEV).view(seqs, -1)
+            lens = [1] * n if seqs > 1 else [n]
+            q = torch.zeros(n, 1, 64, dtype=dtype, device=DEV)
+            q[..., 0] = 1
+            out = dk.paged_attention_varlen(q, cache, cache, tables, int32(lens), int32(starts_of(new)), window=1,
+                                            scale=1.0)
+            assert torch.equal(out[:, 0, 0].float(), v.float()) and torch.equal(out[:, 0, 63].float(), v.float())
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_attention_random_batches(seed):
+    """Any mixture of sizes, features, layouts and types."""
+    g = torch.Generator().manual_seed(1000 + seed)
+    pick = lambda *v: v[int(torch.randint(len(v), (1,), generator=g))]
+    upto = lambda n: int(torch.randint(n, (1,), generator=g))
+    fp8 = upto(3) == 0
+    d = pick(64, 128, 192, 256) if fp8 else pick(64, 96, 128, 192, 256)
+    hkv = pick(1, 2, 3)
+    hq = hkv * pick(1, 2, 3, 5, 8, 16)
+    seqs = pick(1, 2, 5, 9)
+    style = pick("one", "few", "many", "mixed")
+    new = [{"one": upto(2), "few": upto(6), "many": upto(200), "mixed": pick(0, 1, 1, upto(300))}[style] for _ in range(seqs)]
+    top = pick(1, 40, 700, 3000)
+    lens = [max(0, n + upto(top) - (2 if upto(9) == 0 else 0)) for n in new]
+    b = Batch(new, lens, hq, hkv, d, dtype=pick(BF16, FP16), block=pick(1, 8, 16, 16, 32, 40, 48), fp8=fp8,
+              layout=pick("nhd", "hnd", "vllm"), seed=seed)
+    kw = {}
+    if upto(2):
+        kw["window"] = pick(1, 5, 64, 300, 5000)
+    if upto(3) == 0:
+        kw["softcap"] = pick(2.0, 30.0)
+    if upto(3) == 0:
+        kw["alibi_slopes"] = torch.rand(hq, generator=g).to(DEV)
+    if upto(2):
+        kw["prefix_lens"] = int32([upto(100) for _ in new])
+    if b.starts[-1] == 0:
+        return
+    b.check(b.run(**kw), **kw)
+
+
+def test_attention_through_the_c_interface_with_and_without_workspace():
+    L = capi.lib()
+    stream = torch.cuda.current_stream().cuda_stream
+    for new, lens in (([1, 1, 1], [5000, 70, 3000]), ([300, 1], [4000, 2000]), ([3, 2], [2000, 900])):
+        b = Batch(new, lens, 8, 2, 128)
+        out = torch.full_like(b.q, 7.0)
+        dlens, dstarts = int32(lens), int32(b.starts)
+        p = capi.varlen_attn_params(out, b.q, b.k, b.v, b.tables, dlens, dstarts, 128**-0.5, window=1500)
+        args = (capi.dtype_code(BF16), 128, max(new), max(lens))
+        size = L.dk_paged_attention_varlen_workspace_bytes(ctypes.byref(p), *args[1:])
+        assert size > 0
+        ws = torch.full((size // 4 + 64,), float("nan"), device=DEV)  # nothing of it has to be set before
+        guard = ws[size // 4:]
+        guard.fill_(3.0)
+        assert L.dk_paged_attention_varlen(ctypes.byref(p), *args, ws.data_ptr(), size, stream) == 0, capi.last_error()
+        b.check(out, window=1500)
+        assert bool((guard == 3.0).all())
+        assert torch.equal(out, b.run(window=1500))
+        for ptr, have in ((None, 0), (ws.data_ptr(), size - 4)):
+            out.fill_(7.0)
+            assert L.dk_paged_attention_varlen(ctypes.byref(p), *args, ptr, have, stream) == 0, capi.last_error()
+            b.check(out, window=1500)
+
+
+def test_norm_and_slots_through_the_c_interface():
+    L = capi.lib()
+    stream = torch.cuda.current_stream().cuda_stream
+    q, k, v, qw, kw, pos = norm_case(9, 4, 2, 128, 128, True, BF16)
+    table = rope_table(128)
+    r = capi.rotary_params(pos, q, k, 128, table, True)
+    q_out, k_out = (torch.empty(9, h * 128, dtype=BF16, device=DEV) for h in (4, 2))
+    n = capi.qk_norm_params(qw, kw, 1e-6, 128, q_out, k_out)
+    assert L.dk_qk_norm_rotary_embedding(ctypes.byref(r), ctypes.byref(n), capi.DK_BFLOAT16, stream) == 0
+    want = dk.qk_norm_rotary_embedding(pos, q.clone(), k.clone(), qw, kw, 1e-6, 128, table, True)
+    assert torch.equal(q_out, want[0]) and torch.equal(k_out, want[1])
+    kc, vc = (torch.zeros(2, 8, 2, 128, dtype=BF16, device=DEV) for _ in range(2))
+    slots = torch.arange(9, device=DEV) + 3
+    c = capi.cache_write_params(k, v, kc, vc, slots)
+    n = capi.qk_norm_params(qw, kw, 1e-6, 128, q_out.fill_(0))
+    assert L.dk_qk_norm_rotary_embedding_and_cache(ctypes.byref(r), ctypes.byref(n), ctypes.byref(c), capi.DK_BFLOAT16,
+                                                   stream) == 0
+    assert torch.equal(q_out, want[0]) and torch.equal(kc.view(-1, 256)[3:12], want[1])
+    starts, lens, tables = int32([0, 2, 3]), int32([20, 1]), int32([[4, 0], [0, 0]])
+    p64, s64, taken = (torch.empty(3, dtype=t, device=DEV) for t in (torch.int64, torch.int64, torch.int32))
+    s = capi.slot_mapping_params(starts, lens, tables, 16, p64, s64, int32([9, 8, 7]), taken)
+    assert L.dk_build_slot_mapping(ctypes.byref(s), stream) == 0
+    assert p64.tolist() == [18, 19, 0] and taken[0].item() == 1
+    assert s64.tolist() == [2, 3, 9 * 16]  # block 1 of sequence 0 is held: entry 0; sequence 1 takes block 9
 
 
 def test_attention_offsets_past_32_bits():

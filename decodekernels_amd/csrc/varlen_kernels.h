@@ -372,8 +372,9 @@ __device__ __forceinline__ int parts_of(Args& p, int total) {
 template <int D>
 struct TileSmem {
   static constexpr int TK = tile_keys<D>();
-  static constexpr int KP = D + 8;   // row pitches in elements: K rows 4 banks apart, for 16-byte reads of 16 rows;
-  // V rows 16 (8) banks apart, for transpose reads of 64 (32) bytes of 4 rows
+  // Row pitches in elements: K rows 4 (8) banks apart, for 16-byte reads of 32 (16) rows;
+  static constexpr int KP = D + (wave_rows(D) == 32 ? 8 : 16);
+  // V rows 16 (8) banks apart, for transpose reads of 64 (32) bytes of 4 rows.
   static constexpr int VP = D + wave_rows(D);
   struct __attribute__((aligned(16))) Stage {
     uint16_t k[TK * KP];

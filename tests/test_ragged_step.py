@@ -412,6 +412,37 @@ def test_attention_many_sequences():
     b.check(b.run())
 
 
+def test_attention_more_sequences_than_one_scan_takes():
+    g = torch.Generator().manual_seed(2)
+    new = torch.randint(0, 3, (2500,), generator=g).tolist()
+    lens = [n + c for n, c in zip(new, torch.randint(0, 40, (2500,), generator=g).tolist())]
+    b = Batch(new, lens, 2, 1, 64, seed=6)
+    b.check(b.run(max_seq_len=5000))  # cut by shares
+    b.check(b.run())
+    for s in (3, 1023, 1024, 2047, 2048, 2499):
+        new[s], lens[s] = 70, 90 + s % 7
+    b = Batch(new, lens, 2, 1, 64, seed=6)
+    b.check(b.run(max_seq_len=5000))
+
+
+def test_attention_keys_and_values_laid_out_differently():
+    for fp8 in (False, True):
+        b = Batch([1, 90, 3], [700, 300, 50], 4, 2, 128, fp8=fp8)
+        want = b.run()
+        b.check(want)
+        raw = b.v.view(torch.uint8) if fp8 else b.v
+        b.v = raw.transpose(1, 2).contiguous().transpose(1, 2).view(b.v.dtype)
+        assert b.v.stride() != b.k.stride() and torch.equal(b.run(), want)
+
+
+def test_attention_shared_blocks():
+    """Sequences that begin with the same cached blocks, and block size 1 to 100."""
+    for block in (16, 7, 100):
+        b = Batch([1, 40, 2], [400, 440, 402], 4, 2, 128, block=block, poison=False)
+        b.tables[1:, :3 if block < 100 else 1] = b.tables[0, :3 if block < 100 else 1]
+        b.check(b.run())
+
+
 def test_attention_rows_behind_the_last_sequence_stay():
     b = Batch([3, 1, 40], [50, 9, 77], 4, 2, 128)
     q = torch.cat([b.q, torch.full((5, 4, 128), float("nan"), dtype=BF16, device=DEV)])

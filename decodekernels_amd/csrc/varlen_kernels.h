@@ -41,16 +41,16 @@ struct KParams {
   int max_len;             // no length goes past it: the caller's bound, and what the tables can hold
   int window;              // keys a token sees, itself included; max_len where it sees all before it
   int hkv;
-  int split_items;         // tile_kernel: workgroups that the tiles of a call may be split over; 0: never split
-  int shares;              // row_kernel: workgroups a KV head, of equal shares of all key tiles; 0: one a sequence
+  int split_items;         // tile_work: workgroups that the tiles of a call may be split over; 0: never split
+  int shares;              // row_work: workgroups a KV head, of equal shares of all key tiles; 0: one a sequence
   int tile_groups;         // workgroups of tile_work
   int row_from;            // the first workgroup of row_work
-  int short_rows;          // rows of a KV head up to which a sequence runs in row_kernel: 16 or 32
-  int slot_rows;           // row_kernel: rows of a slot, as many as max_query_len allows
+  int short_rows;          // rows of a KV head up to which a sequence runs in row_work: 16 or 32
+  int slot_rows;           // row_work: rows of a slot, as many as max_query_len allows
   // Partial results, row by row of an item or slot: sums, and their reference
   // maximum (log2 units) and exp-sum.
   float *tile_ws, *tile_ml, *ws, *ws_ml;
-  int32_t* ws_first;       // row_kernel: a sequence's first workgroup, and how many
+  int32_t* ws_first;       // row_work: a sequence's first workgroup, and how many
   uint32_t bs_mul;         // j / block_size = (j * bs_mul) >> bs_shift, for j < 2^31
   int bs_shift;
   int biased;              // slopes are given
@@ -118,7 +118,10 @@ constexpr int kWholeKeys = 512, kWholeKeysMany = 2048, kManyPairs = 192;
 // workgroup (48 speculating sequences of 200-8000 keys: 66.8 us with 8, 62.5 with
 // 32; twice the share is too many: 32 sequences of 500-8000 keys 105 and 134 us).
 constexpr int kMinShare = 8, kMorePart = 32;
-constexpr int kMinPart = 8;     // key tiles of a part of a row tile at least
+// Key tiles of a part of a row tile at least, so that its sums' way through
+// memory stays small against it. (4, 8 and 16 measured the same within 1% at a
+// 512-token chunk on 16000 keys and beside 32 decoding sequences.)
+constexpr int kMinPart = 8;
 constexpr int kWideRows = 192;  // head_dim up to which 32 rows share a reading: 256 has no registers for them
 
 // Infinities and NaN of the dtype: the exponent bits of an element, and the
@@ -395,7 +398,15 @@ struct TileSmem {
 // maximum and sum of a row need one exchange (two), and the weights are, rounded
 // to the dtype, the B operand of O^T = V^T P^T as they stand, with V^T read
 // transposed from LDS. O^T has its row in the same lane again, so rescaling is
-// a multiplication.
+// a multiplication. Two key tiles are in flight: one in LDS under the products,
+// the next in registers.
+//
+// Bound by a wave's own chain of products, exponentials and LDS reads at two
+// waves a SIMD (LDS and registers allow no third): at two prompts of 8192 tokens,
+// 32 / 8 heads of 128, the matrix units are busy 42% of the time, the vector units 42%
+// and LDS 32%; 1.18 ms, 935 TFLOP/s of the 1360 that a large product reaches.
+// Heads of 256: 0.28 ms for nine prompts of 134 GFLOP (vector units 37%, LDS 34%,
+// matrix units 22%).
 template <typename E, int D>
 struct TileMath {
   static constexpr int WR = wave_rows(D);
@@ -798,7 +809,7 @@ __global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2,
   tile_work<E, D, FP8, BS16>(fresh_args(), sm);
 }
 
-// Joins the parts of row tiles over which tile_kernel was spread, in their
+// Joins the parts of row tiles over which tile_work was spread, in their
 // order. Workgroup (x, y) takes 16 rows of tile x / hkv, KV head x % hkv.
 template <typename E, int D>
 __global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams) {
@@ -848,7 +859,7 @@ __global__ __launch_bounds__(kTileThreads) void tile_join_kernel(const KParams) 
   }
 }
 
-// LDS of row_kernel: each wave's current key tile, then, at the end of a piece,
+// LDS of row_work: each wave's current key tile, then, at the end of a piece,
 // the waves' sums in the same place.
 template <int D, int R, bool FP8>
 struct RowSmem {
@@ -881,6 +892,11 @@ constexpr int row_occupancy() {  // waves per SIMD
 // not a whole sequence leaves its sums in slot g + s (sequence s; no two pieces
 // share one) for row_join_kernel. Scores are S^T = K Q^T and the output O^T =
 // V^T P^T on 16x16 MFMAs: lane l holds rows l % 16 (and + 16) of both.
+// 64 sequences of 605 MB in all: 103 us, 5.8 TB/s with the joining launch; one
+// of 128K keys (537 MB) 92 us; 32 with windows (68 MB) 23 us, of which joining
+// and the second launch are 5; 48 speculating over 203 MB of fp8: 58 us (two
+// waves a SIMD that wait for their own loads and LDS writes: vector units 32%
+// busy, LDS 33%, matrix units 13%).
 template <typename E, int D, int R, bool FP8, bool BS16, typename Params>
 __device__ __forceinline__ void row_work(const Params& p, RowSmem<D, R, FP8>& sm) {
   using Smem = RowSmem<D, R, FP8>;
@@ -1365,7 +1381,7 @@ __global__ __launch_bounds__(kTileThreads) __attribute__((amdgpu_waves_per_eu(2,
     row_work<E, D, 1, FP8, BS16>(fresh_args(), *reinterpret_cast<RowSmem<D, 1, FP8>*>(raw));
 }
 
-// Joins the pieces of row_kernel's cut sequences, in their order: a wave a row.
+// Joins the pieces of row_work's cut sequences, in their order: a wave a row.
 template <typename E, int D>
 __global__ __launch_bounds__(kTileThreads) void row_join_kernel(const KParams p) {
   constexpr int LD = D / 4;                        // lanes of a row

@@ -5,11 +5,13 @@ defaults and errors) over this package's HIP kernels. The raw ops
 ``torch.ops.decode_kernels.*`` mutate their ``Tensor!`` arguments and can run
 on preallocated buffers inside a HIP graph; these wrappers allocate outputs
 (and the attention split-K workspace) when the caller does not pass them. All
-raw ops but one allocate nothing. ``gemm_tn``, unlike the reference's op, takes
-the fp32 workspace of the decode shapes whose plan splits K (splits * M * N * 4
-bytes) from PyTorch's caching allocator, stream-ordered, so it still captures
-in a graph (private pool). The C ABI's ``dk_gemm_tn_ws`` with a caller
-workspace is the allocation-free route.
+raw ops but two kinds allocate nothing. ``gemm_tn``, unlike the reference's op,
+takes the fp32 workspace of the decode shapes whose plan splits K (splits * M *
+N * 4 bytes) from PyTorch's caching allocator, and ``paged_attention_varlen``
+(and its fp8 form) that of keys split over workgroups; stream-ordered, so both
+still capture in a graph (private pool). The C ABI's ``dk_gemm_tn_ws`` and
+``dk_paged_attention_varlen`` with a caller workspace are the allocation-free
+route.
 """
 
 from __future__ import annotations

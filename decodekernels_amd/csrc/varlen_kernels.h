@@ -375,13 +375,17 @@ __device__ __forceinline__ int parts_of(Args& p, int total) {
 template <int D>
 struct TileSmem {
   static constexpr int TK = tile_keys<D>();
-  // Row pitches in elements: K rows 4 (8) banks apart, for 16-byte reads of 32 (16) rows;
-  static constexpr int KP = D + (wave_rows(D) == 32 ? 8 : 16);
-  // V rows 16 (8) banks apart, for transpose reads of 64 (32) bytes of 4 rows.
-  static constexpr int VP = D + wave_rows(D);
+  // Rows lie next to one another (loads straight to LDS fill 1 KB in lane order),
+  // with the 16-byte chunk c of row r in the place of c ^ k_swap(r), c ^ v_swap(r):
+  // reads of one chunk of 16 K rows, and transpose reads of 64 (32) bytes of 4 (8)
+  // V rows, take all 64 banks.
+  static constexpr int M = D / 8 % 16 == 0 ? 16 : D / 8 % 8 == 0 ? 8 : 4;  // chunks a swap stays within
+  static constexpr int G = wave_rows(D) / 8;                               // chunks of a transpose read
+  static __device__ __forceinline__ int k_swap(int r) { return r / (16 / M) % M; }
+  static __device__ __forceinline__ int v_swap(int r) { return r / (16 / M) % (M / G) * G; }
   struct __attribute__((aligned(16))) Stage {
-    uint16_t k[TK * KP];
-    uint16_t v[TK * VP];
+    uint16_t k[TK * D];
+    uint16_t v[TK * D];
   } stage[2];
   // Infinities and NaN taken out of a stage's V rows: whether a wave's rows had
   // any, and then a bit for each column (infinity or NaN; minus infinity or NaN).
@@ -398,8 +402,8 @@ struct TileSmem {
 // maximum and sum of a row need one exchange (two), and the weights are, rounded
 // to the dtype, the B operand of O^T = V^T P^T as they stand, with V^T read
 // transposed from LDS. O^T has its row in the same lane again, so rescaling is
-// a multiplication. Two key tiles are in flight: one in LDS under the products,
-// the next in registers.
+// a multiplication. Two key tiles are in LDS: one under the products, the next
+// on its way.
 //
 // Bound by a wave's own chain of products, exponentials and LDS reads at two
 // waves a SIMD (LDS and registers allow no third): at two prompts of 8192 tokens,
@@ -431,7 +435,7 @@ struct TileMath {
 template <typename E, int D, bool FP8, bool BS16>
 __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
   using Smem = TileSmem<D>;
-  constexpr int TK = Smem::TK, KP = Smem::KP, VP = Smem::VP;
+  constexpr int TK = Smem::TK, G = Smem::G;
   using Math = TileMath<E, D>;
   using Acc = typename Math::acc_t;
   constexpr int WR = Math::WR;
@@ -508,6 +512,13 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
   // Row and column of this lane's chunks in the wave's RW key rows.
   auto chunk_row = [&](int i) { return kWave % CPR == 0 ? lane / CPR + i * (kWave / CPR) : (lane + kWave * i) / CPR; };
   auto chunk_col = [&](int i) { return 8 * (kWave % CPR == 0 ? lane % CPR : (lane + kWave * i) % CPR); };
+  // The columns that belong there.
+  auto k_col = [&](int i) { return chunk_col(i) ^ 8 * Smem::k_swap(RW * wave + chunk_row(i)); };
+  auto v_col = [&](int i) { return chunk_col(i) ^ 8 * Smem::v_swap(RW * wave + chunk_row(i)); };
+  // Tiles go to LDS past the registers where 16 keys lie in one cache block and
+  // need no conversion (cold, through registers and past them: two prompts of 8192
+  // tokens 1157 and 1091 us, four of 2000 with heads of 256 260 and 223).
+  constexpr bool DIRECT = BS16 && !FP8;
   Chunk rk[NI], rv[NI];
 
   const char* kbase = static_cast<const char*>(p.k) + ELT * (static_cast<int64_t>(kv_head) * p.k_sh);
@@ -517,7 +528,7 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
   auto used = [&](int j) { return in_ranges(j, sq.pre, lo, hi); };
   auto page_of = [&](int t) { return min(max(t, 0), p.num_blocks - 1); };
 
-  auto load = [&](int n) {
+  auto load = [&](int n, [[maybe_unused]] typename Smem::Stage* to) {
     const int t0 = tiles.index(n) * TK;
     const int r0 = t0 + RW * wave;
     const int all = t0 + TK <= sq.pre || (t0 >= lo && t0 + TK <= hi) ? -1 : 0;  // every key of the tile
@@ -541,14 +552,16 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
       }
 #pragma unroll
       for (int i = 0; i < NI; ++i) {
-        const int ko = hide[i] | ELT * (chunk_row(i) * p.k_st + chunk_col(i));
-        const int vo = hide[i] | ELT * (chunk_row(i) * p.v_st + chunk_col(i));
-        if constexpr (FP8) {
+        const int ko = hide[i] | ELT * (chunk_row(i) * p.k_st + k_col(i));
+        const int vo = hide[i] | ELT * (chunk_row(i) * p.v_st + v_col(i));
+        if constexpr (DIRECT) {
+          using lds_ptr = __attribute__((address_space(3))) void*;
+          const int at = RW * wave * D + 8 * kWave * i;  // and 16 bytes a lane from there
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(brk, (lds_ptr)(to->k + at), 16, ko, 0, 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(brv, (lds_ptr)(to->v + at), 16, vo, 0, 0, 0);
+        } else {
           rk[i] = __builtin_amdgcn_raw_buffer_load_b64(brk, ko, 0, 0);
           rv[i] = __builtin_amdgcn_raw_buffer_load_b64(brv, vo, 0, 0);
-        } else {
-          rk[i] = __builtin_amdgcn_raw_buffer_load_b128(brk, ko, 0, 0);
-          rv[i] = __builtin_amdgcn_raw_buffer_load_b128(brv, vo, 0, 0);
         }
       }
     } else {
@@ -560,8 +573,8 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
           const int blk = div_block(p, j);
           const int64_t page = page_of(p.tables[table_row + blk]);
           const int64_t off = j - blk * p.block_size;
-          rk[i] = *reinterpret_cast<const Chunk*>(kbase + ELT * (page * p.k_sb + off * p.k_st + chunk_col(i)));
-          rv[i] = *reinterpret_cast<const Chunk*>(vbase + ELT * (page * p.v_sb + off * p.v_st + chunk_col(i)));
+          rk[i] = *reinterpret_cast<const Chunk*>(kbase + ELT * (page * p.k_sb + off * p.k_st + k_col(i)));
+          rv[i] = *reinterpret_cast<const Chunk*>(vbase + ELT * (page * p.v_sb + off * p.v_st + v_col(i)));
         }
       }
     }
@@ -569,13 +582,24 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
   // Every row of the workgroup sees all keys of the tile.
   auto all_see = [&](int t0) { return t0 + TK <= sq.pre || (t0 + TK - 1 <= pos0 && t0 > pos1 - p.window); };
   auto store = [&](int n, int st) {
+    const bool look = !all_see(tiles.index(n) * TK);
+    auto place = [&](uint16_t* stage, int i) {
+      return reinterpret_cast<u32x4*>(stage + (RW * wave + chunk_row(i)) * D + chunk_col(i));
+    };
     u32x4 v[NI];
+    if constexpr (DIRECT) {
+      __builtin_amdgcn_s_waitcnt((7 << 4) | (15 << 8));  // vmcnt(0): this wave's rows are in LDS
+      if (!look) return;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      if constexpr (FP8) v[i] = fp8x8_to<E>(rv[i]);
-      else v[i] = rv[i];
+      for (int i = 0; i < NI; ++i) v[i] = *place(sm.stage[st].v, i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        if constexpr (FP8) v[i] = fp8x8_to<E>(rv[i]);
+        else v[i] = rv[i];
+      }
     }
-    if (!all_see(tiles.index(n) * TK)) {
+    if (look) {
       u16x2 open = {0xffff, 0xffff};
 #pragma unroll
       for (int i = 0; i < NI; ++i) open = fold_finite<E>(open, v[i]);
@@ -587,18 +611,18 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
           uint32_t up, down;
           v[i] = take_out<E>(v[i], up, down);
           const int r = RW * wave + chunk_row(i);
-          reinterpret_cast<uint8_t*>(sm.up[st][r])[chunk_col(i) / 8] = static_cast<uint8_t>(up);
-          reinterpret_cast<uint8_t*>(sm.down[st][r])[chunk_col(i) / 8] = static_cast<uint8_t>(down);
+          reinterpret_cast<uint8_t*>(sm.up[st][r])[v_col(i) / 8] = static_cast<uint8_t>(up);
+          reinterpret_cast<uint8_t*>(sm.down[st][r])[v_col(i) / 8] = static_cast<uint8_t>(down);
+          if constexpr (DIRECT) *place(sm.stage[st].v, i) = v[i];
         }
       }
     }
+    if constexpr (DIRECT) return;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = RW * wave + chunk_row(i);
-      u32x4* k = reinterpret_cast<u32x4*>(sm.stage[st].k + r * KP + chunk_col(i));
-      if constexpr (FP8) *k = fp8x8_to<E>(rk[i]);
-      else *k = rk[i];
-      *reinterpret_cast<u32x4*>(sm.stage[st].v + r * VP + chunk_col(i)) = v[i];
+      if constexpr (FP8) *place(sm.stage[st].k, i) = fp8x8_to<E>(rk[i]);
+      else *place(sm.stage[st].k, i) = rk[i];
+      *place(sm.stage[st].v, i) = v[i];
     }
   };
 
@@ -608,19 +632,20 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
   float m_ref = -__builtin_huge_valf();  // log2 units
   float l_run = 0.0f;                    // this lane's share of the row's sum
 
-  auto compute = [&](int n, int st) {
+  auto compute = [&](int n, int st, const typename Smem::Stage* from) {
     const int t0 = tiles.index(n) * TK;
     // Seen by no row of this wave / by all of them.
     if (!wave_live || (t0 >= sq.pre && (t0 > wpos1 || t0 + TK <= wpos0 - p.window + 1))) return;
     const bool full = t0 + TK <= sq.pre || (t0 + TK - 1 <= wpos0 && t0 > wpos1 - p.window);
     Acc s[KB];
-    const uint16_t* kt = sm.stage[st].k + lr * KP + 2 * part4;
+    const uint16_t* kt = from->k + lr * D;
+    const int kc = 2 * part4 ^ 8 * Smem::k_swap(lr);
 #pragma unroll
     for (int b = 0; b < KB; ++b) {
       s[b] = Acc{};
 #pragma unroll
       for (int c = 0; c < KS; ++c) {
-        const u32x4 ka = *reinterpret_cast<const u32x4*>(kt + WR * b * KP + CS * c);
+        const u32x4 ka = *reinterpret_cast<const u32x4*>(kt + WR * b * D + (CS * c ^ kc));
         s[b] = Math::mma(ka, qf[c], s[b]);
       }
     }
@@ -702,15 +727,15 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
         l_run += x + y;
         pk[(NE * b + i) / 8][(NE * b + i) % 8 / 2] = pack2<E>(x, y);
       }
-    const uint16_t* vt =
-        sm.stage[st].v + (part4 + (lane % 16) / 4) * VP + (WR == 32 ? 16 * ((lane / 16) % 2) : 0) + 4 * (lane % 4);
+    const int vr = part4 + (lane % 16) / 4, vc = 8 * Smem::v_swap(vr);
+    const uint16_t* vt = from->v + vr * D + (WR == 32 ? 16 * ((lane / 16) % 2) : 0) + 4 * (lane % 4);
     // A operand of O^T: columns WR b + lr, the keys of step c in the order of pk[c].
     auto v_operand = [&](int c, int b) {
       using lds_v4i16 = __attribute__((address_space(3))) s16x4;
       const u32x2 x = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + CS * c * VP + WR * b)));
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + CS * c * D + (WR * b ^ vc))));
       const u32x2 y = __builtin_bit_cast(
-          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + (CS * c + CS / 2) * VP + WR * b)));
+          u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4i16*)(vt + (CS * c + CS / 2) * D + (WR * b ^ vc))));
       return u32x4{x[0], x[1], y[0], y[1]};
     };
 #pragma unroll
@@ -760,14 +785,20 @@ __device__ __forceinline__ void tile_work(Args& p, TileSmem<D>& sm) {
     }
   };
 
+  // (restrict: reads of one stage need not wait for loads to the other, which the
+  // compiler otherwise makes them: one prompt of 2048 tokens 67.6 us, and 76.2 so.)
+  auto step = [&](int n, int st, const typename Smem::Stage* __restrict__ from, typename Smem::Stage* __restrict__ to) {
+    if (n + 1 < n1) load(n + 1, to);
+    compute(n, st, from);
+  };
+
   if (n0 < n1) {
-    load(n0);
+    load(n0, sm.stage);
     store(n0, 0);
     lds_barrier();
     for (int n = n0; n < n1; ++n) {
       const int st = (n - n0) & 1;
-      if (n + 1 < n1) load(n + 1);
-      compute(n, st);
+      step(n, st, sm.stage + st, sm.stage + (st ^ 1));
       if (n + 1 < n1) store(n + 1, st ^ 1);
       lds_barrier();
     }

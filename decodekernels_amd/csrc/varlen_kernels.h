@@ -407,10 +407,10 @@ struct TileSmem {
 //
 // Bound by a wave's own chain of products, exponentials and LDS reads at two
 // waves a SIMD (LDS and registers allow no third): at two prompts of 8192 tokens,
-// 32 / 8 heads of 128, the matrix units are busy 42% of the time, the vector units 42%
-// and LDS 32%; 1.18 ms, 935 TFLOP/s of the 1360 that a large product reaches.
-// Heads of 256: 0.28 ms for nine prompts of 134 GFLOP (vector units 37%, LDS 34%,
-// matrix units 22%).
+// 32 / 8 heads of 128, the matrix units are busy 49% of the time, the vector units 47%
+// and LDS 25%; 1.11 ms, 987 TFLOP/s of the 1360 that a large product reaches.
+// Heads of 256: 0.25 ms for nine prompts of 134 GFLOP (vector units 41%, LDS 26%,
+// matrix units 25%).
 template <typename E, int D>
 struct TileMath {
   static constexpr int WR = wave_rows(D);
@@ -925,7 +925,7 @@ constexpr int row_occupancy() {  // waves per SIMD
 // V^T P^T on 16x16 MFMAs: lane l holds rows l % 16 (and + 16) of both.
 // 64 sequences of 605 MB in all: 103 us, 5.8 TB/s with the joining launch; one
 // of 128K keys (537 MB) 92 us; 32 with windows (68 MB) 23 us, of which joining
-// and the second launch are 5; 48 speculating over 203 MB of fp8: 58 us (two
+// and the second launch are 5; 48 speculating over 203 MB of fp8: 56 us (two
 // waves a SIMD that wait for their own loads and LDS writes: vector units 32%
 // busy, LDS 33%, matrix units 13%).
 template <typename E, int D, int R, bool FP8, bool BS16, typename Params>
